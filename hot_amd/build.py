@@ -14,7 +14,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 OUT = os.path.join(HERE, 'libhotk.so')
 OBJ = os.path.join(HERE, 'csrc', '_obj')
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Wno-unused-value',
-         '-mllvm', '-amdgpu-mfma-vgpr-form']   # MFMA results in VGPRs: no v_accvgpr_read/write around the tile code
+         '-mllvm', '-amdgpu-mfma-vgpr-form',   # MFMA results in VGPRs: no v_accvgpr_read/write around the tile code
+         # no packed fp32 arithmetic: -O3 forms v_pk_{add,mul,fma}_f32 from ordinary float code by itself, and some of their
+         # operand forms have given wrong results now and then (the host pass warns that it does not know the feature)
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def sources():
