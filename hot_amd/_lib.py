@@ -114,6 +114,30 @@ _SIGNATURES.update({
     'hotk_assemble22_bf16': [_P, _L, _P, _L, _P, _P, _P, _P, _P, _L, _L, _P],
     'hotk_seg_sum_rows_bf16': [_P, _L, _P, _P, _P, _P, _U, _P, _L, _L, _L, _L, _P],
 })
+
+
+class LinearArgs(ctypes.Structure):
+    """mirror of hotk_linear_args (include/hotk.h)"""
+    _fields_ = [('M', _L), ('N', _L), ('K', _L), ('x', _P), ('ld_x', _L), ('w', _P), ('ld_w', _L), ('bias', _P), ('res', _P),
+                ('ld_res', _L), ('y', _P), ('ld_y', _L), ('save', _P), ('x_scale', _P), ('w_scale', _P),
+                ('type', ctypes.c_int32), ('out_type', ctypes.c_int32), ('act', ctypes.c_int32), ('reserved', ctypes.c_int32)]
+
+
+TYPE_F32, TYPE_BF16, TYPE_F16, TYPE_E4M3 = range(4)
+ACTS = {'none': 0, 'relu': 1, 'leakyrelu': 2, 'gelu': 3, 'tanh': 4, 'silu': 5}
+
+_SIGNATURES.update({
+    'hotk_rmsnorm_supported': [_L, _I],
+    'hotk_rmsnorm_fwd': [_P, _L, _P, _L, _P, _P, _U, _F, _P, _P, _P, _L, _L, _I, _P],
+    'hotk_rmsnorm_quant': [_P, _L, _P, _L, _P, _P, _U, _F, _P, _P, _P, _L, _L, _I, _P],
+    'hotk_quantize_rows': [_P, _L, _P, _P, _L, _L, _I, _P],
+    'hotk_rmsnorm_partials': [_L, _L, _I, ctypes.POINTER(_L)],
+    'hotk_rmsnorm_bwd': [_P, _L, _P, _L, _P, _L, _P, _P, _P, _U, _P, _P, _L, _L, _I, _P],
+    'hotk_sum_partials': [_P, _L, _L, _P, _I, _P],
+    'hotk_linear_workspace_bytes': [_L, _L, _L, _I, ctypes.POINTER(_S)],
+    'hotk_linear_act': [ctypes.POINTER(LinearArgs), _P, _S, _P],
+    'hotk_linear_turn': [_P, _L, _P, _I, _P, _L, _P, _L, _P, _L, _L, _I, _P],
+})
 EXPORTS = sorted(list(_SIGNATURES) + ['hotk_strerror', 'hotk_version'])
 
 _lib = None

@@ -1,0 +1,451 @@
+// Root-mean-square norm of a residual stream, its 8-bit form, and rows to 8 bits (the norm and the operand makers of the
+// feed-forward block; the product that reads them is in linact.hip).
+//
+//   h = round(x + r)                   the stream as it is stored; without a residual h = x
+//   rstd = (mean_c h^2 + eps)^(-1/2)   y = h * rstd * w
+//   backward, u = h * rstd, g = dy * w:   dx = dr = rstd * (g - u * mean_c(g u)) + dh,   dw = sum_r dy * u
+//   8 bits:  scale = max(max_c |y| / 448, 2^-126),   q = e4m3(y / scale)
+//   rows that `keep` leaves out: h, y, q and dx are zero and nothing of the row is read
+//
+// Everything between the load and the one rounding at the store is in 32 bits; the norm reads the ROUNDED h, so that the
+// backward pass, which finds h and not x and r, differentiates what the forward pass computed.
+//
+// A group of WPR waves owns a row and holds it in registers, VEC elements (16 bytes) a lane and NV of them, so a row is read
+// once.  Sums cross lanes by shuffles and waves through LDS.  HBM-bound.  A row that is no multiple of VEC has no tail: the
+// last piece starts VEC before its end, overlapping its neighbour (and so do the lanes past the end); the sums count each
+// element in one lane only, the stores write the same values twice.  Rows shorter than VEC go element by element (SMALL).
+#include "ffn.h"
+
+namespace {
+
+constexpr int RN_MAX_D = 32768;
+constexpr float RN_E4M3_MAX = 448.f;
+constexpr float RN_SCALE_MIN = 0x1p-126f;
+
+__device__ __forceinline__ float rn_wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// the largest magnitude as the bits of a non-negative float: integer order is float order there, and a NaN is above infinity
+__device__ __forceinline__ uint32_t rn_wave_max(uint32_t v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const uint32_t t = (uint32_t)__shfl_xor((int)v, o, 64);
+    v = t > v ? t : v;
+  }
+  return v;
+}
+// over the WPR waves of a row's group.  `slot` alternates between calls: one barrier per call is enough, since a wave that
+// writes a slot again has passed the barrier of the call in between, which every reader reached after its reads.
+template <int WPR>
+__device__ __forceinline__ float rn_group_sum(float v, float (*box)[16], int& slot, int w) {
+  v = rn_wave_sum(v);
+  if (WPR == 1) return v;
+  if ((threadIdx.x & 63) == 0) box[slot][w] = v;
+  __syncthreads();
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < WPR; ++i) t += box[slot][i];
+  slot ^= 1;
+  return t;
+}
+template <int WPR>
+__device__ __forceinline__ uint32_t rn_group_max(uint32_t v, float (*box)[16], int& slot, int w) {
+  v = rn_wave_max(v);
+  if (WPR == 1) return v;
+  if ((threadIdx.x & 63) == 0) box[slot][w] = __uint_as_float(v);
+  __syncthreads();
+  uint32_t t = 0;
+#pragma unroll
+  for (int i = 0; i < WPR; ++i) {
+    const uint32_t u = __float_as_uint(box[slot][i]);
+    t = u > t ? u : t;
+  }
+  slot ^= 1;
+  return t;
+}
+
+// ---- a lane's piece of a row --------------------------------------------------------------------------------------------
+template <class T, bool SMALL>
+struct Piece {
+  using E = Elem<T>;
+  using FV = typename E::fvec;
+  int c;          // first column
+  int skip;       // leading elements that belong to a neighbour (VEC: the whole piece); SMALL: unused
+  __device__ __forceinline__ Piece(int lane, int D) {
+    const int want = E::VEC * lane;
+    if (SMALL) {
+      c = want;
+      skip = 0;
+    } else {
+      c = want < D - E::VEC ? want : D - E::VEC;
+      skip = want < D ? want - c : E::VEC;
+    }
+  }
+  __device__ __forceinline__ bool mine(int k, int D) const { return SMALL ? c + k < D : k >= skip; }
+  __device__ __forceinline__ FV load(const T* __restrict__ row, int D) const {
+    if (SMALL) return ffn_load(row, c, D);
+    return __builtin_convertvector((typename E::vec)(*reinterpret_cast<const typename E::uvec*>(row + c)), FV);
+  }
+  __device__ __forceinline__ bool any(int D) const { return SMALL ? c < D : skip < E::VEC; }
+  __device__ __forceinline__ void store(T* __restrict__ row, int D, FV v) const {
+    if (!any(D)) return;
+    if (SMALL) ffn_store(row, c, D, v);
+    else *reinterpret_cast<typename E::uvec*>(row + c) = __builtin_convertvector(v, typename E::vec);
+  }
+  // rounded to e4m3
+  __device__ __forceinline__ void store8(uint8_t* __restrict__ row, int D, FV v) const {
+    if (!any(D)) return;
+    uint32_t b[E::VEC / 4];
+#pragma unroll
+    for (int i = 0; i < E::VEC / 4; ++i) {
+      const int t = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i], v[4 * i + 1], 0, false);
+      b[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2], v[4 * i + 3], t, true);
+    }
+    if (SMALL) {
+#pragma unroll
+      for (int i = 0; i < E::VEC; ++i)
+        if (c + i < D) row[c + i] = (uint8_t)(b[i / 4] >> (8 * (i % 4)));
+    } else {
+      __builtin_memcpy(row + c, b, E::VEC);
+    }
+  }
+};
+
+template <class T>
+struct RnFwd {
+  const T *x, *r, *w;
+  int64_t ld_x, ld_r;
+  const uint8_t* kind;
+  unsigned keep;
+  float eps;
+  T *y, *h;
+  float* rstd;
+  uint8_t* q;
+  float* scale;
+  int64_t R;
+  int D;
+};
+
+enum { RN_NORM = 0, RN_NORM8 = 1, RN_QUANT = 2 };
+
+template <class T, int MODE, int NV, int WPR, int WAVES, bool SMALL>
+__global__ __launch_bounds__(64 * WAVES) void k_rmsnorm_fwd(const RnFwd<T> a) {
+  using E = Elem<T>;
+  using FV = typename E::fvec;
+  constexpr int VEC = E::VEC, GROUPS = WAVES / WPR, LANES = 64 * WPR;
+  static_assert(WPR == 1 || GROUPS == 1, "a row's group is one wave or the whole workgroup (barriers)");
+  __shared__ float box[2][16];
+  int slot = 0;
+  const int wave = threadIdx.x >> 6;
+  const int t = WPR == 1 ? (threadIdx.x & 63) : threadIdx.x;
+  const int D = a.D;
+  for (int64_t row = (int64_t)blockIdx.x * GROUPS + (WPR == 1 ? wave : 0); row < a.R; row += (int64_t)gridDim.x * GROUPS) {
+    const bool kept = !a.kind || hotk_keep(a.keep, a.kind[row]);
+    FV v[NV];
+    if (kept) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) v[i] = Piece<T, SMALL>(t + LANES * i, D).load(a.x + row * a.ld_x, D);
+      if (MODE != RN_QUANT && a.r) {
+        FV r[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) r[i] = Piece<T, SMALL>(t + LANES * i, D).load(a.r + row * a.ld_r, D);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)      // what the norm reads is what is stored
+          v[i] = __builtin_convertvector(__builtin_convertvector(v[i] + r[i], typename E::vec), FV);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) v[i] = 0.f;
+    }
+    if (MODE != RN_QUANT) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const Piece<T, SMALL> p(t + LANES * i, D);
+        if (a.r) p.store(a.h + row * D, D, v[i]);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) s += p.mine(k, D) ? v[i][k] * v[i][k] : 0.f;
+      }
+      const float rstd = rsqrtf(rn_group_sum<WPR>(s, box, slot, wave) / (float)D + a.eps);
+      if (a.rstd && t == 0) a.rstd[row] = rstd;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const Piece<T, SMALL> p(t + LANES * i, D);
+        v[i] = v[i] * rstd * p.load(a.w, D);
+        if (!kept) v[i] = 0.f;            // (an infinite weight times zero)
+        if (MODE == RN_NORM) p.store(a.y + row * D, D, v[i]);
+      }
+    }
+    if (MODE != RN_NORM) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {   // (SMALL: the elements past the end are zeros; else a lane past the end repeats others)
+          const uint32_t u = __float_as_uint(v[i][k]) & 0x7fffffffu;
+          m = u > m ? u : m;
+        }
+      float scale = __uint_as_float(rn_group_max<WPR>(m, box, slot, wave)) / RN_E4M3_MAX;
+      scale = scale < RN_SCALE_MIN ? RN_SCALE_MIN : scale;     // (a NaN stays one)
+      if (t == 0) a.scale[row] = scale;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) Piece<T, SMALL>(t + LANES * i, D).store8(a.q + row * D, D, v[i] / scale);
+    }
+  }
+}
+
+template <class T>
+struct RnBwd {
+  const T *dy, *dh, *h, *w;
+  int64_t ld_dy, ld_dh, ld_h;
+  const float* rstd;
+  const uint8_t* kind;
+  unsigned keep;
+  T* dx;
+  float* partial;
+  int64_t R;
+  int D;
+};
+
+template <class T, int NV, int WPR, int WAVES, bool SMALL>
+__global__ __launch_bounds__(64 * WAVES) void k_rmsnorm_bwd(const RnBwd<T> a) {
+  using E = Elem<T>;
+  using FV = typename E::fvec;
+  constexpr int VEC = E::VEC, GROUPS = WAVES / WPR, LANES = 64 * WPR;
+  static_assert(WPR == 1 || GROUPS == 1, "a row's group is one wave or the whole workgroup (barriers)");
+  __shared__ float box[2][16];
+  __shared__ FV fold[GROUPS][64];
+  int slot = 0;
+  const int wave = threadIdx.x >> 6;
+  const int t = WPR == 1 ? (threadIdx.x & 63) : threadIdx.x;
+  const int D = a.D;
+  const float inv_d = 1.f / (float)D;
+  FV dw[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) dw[i] = 0.f;
+  for (int64_t row = (int64_t)blockIdx.x * GROUPS + (WPR == 1 ? wave : 0); row < a.R; row += (int64_t)gridDim.x * GROUPS) {
+    if (a.kind && !hotk_keep(a.keep, a.kind[row])) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) Piece<T, SMALL>(t + LANES * i, D).store(a.dx + row * D, D, (FV)0.f);
+      continue;
+    }
+    const float rstd = a.rstd[row];
+    FV g[NV], u[NV];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const Piece<T, SMALL> p(t + LANES * i, D);
+      g[i] = p.load(a.dy + row * a.ld_dy, D);
+      u[i] = p.load(a.h + row * a.ld_h, D);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const Piece<T, SMALL> p(t + LANES * i, D);
+      u[i] *= rstd;
+      dw[i] += g[i] * u[i];
+      g[i] *= p.load(a.w, D);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s += p.mine(k, D) ? g[i][k] * u[i][k] : 0.f;
+    }
+    const float m = rn_group_sum<WPR>(s, box, slot, wave) * inv_d;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const Piece<T, SMALL> p(t + LANES * i, D);
+      FV o = rstd * (g[i] - u[i] * m);
+      if (a.dh) o += p.load(a.dh + row * a.ld_dh, D);
+      p.store(a.dx + row * D, D, o);
+    }
+  }
+  // one partial row of dw per workgroup: a group's lanes own their columns, the waves of WPR = 1 are added in wave order
+  float* out = a.partial + (int64_t)blockIdx.x * D;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const Piece<T, SMALL> p(t + LANES * i, D);
+    FV o = dw[i];
+    if (GROUPS > 1) {
+      __syncthreads();
+      fold[wave][t] = o;
+      __syncthreads();
+      if (wave != 0) continue;
+#pragma unroll
+      for (int w = 1; w < GROUPS; ++w) o += fold[w][t];
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k)
+      if (p.mine(k, D)) out[p.c + k] = o[k];
+  }
+}
+
+// out[c] = sum over b of partial[b][c], in an order that the sizes alone set: a wave adds every 16th row, the sixteen are
+// joined in order
+constexpr int SP_WAVES = 16;
+template <class T>
+__global__ __launch_bounds__(64 * SP_WAVES) void k_sum_partials(const float* __restrict__ partial, int64_t n, int64_t D,
+                                                                T* __restrict__ out) {
+  __shared__ float part[SP_WAVES][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (c < D)
+    for (int64_t b = wave; b < n; b += SP_WAVES) s += partial[b * D + c];
+  part[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && c < D) {
+#pragma unroll
+    for (int w = 1; w < SP_WAVES; ++w) s += part[w][lane];
+    out[c] = (T)s;
+  }
+}
+
+unsigned rn_grid(int64_t rows, int groups, unsigned cap) {
+  const int64_t g = (rows + groups - 1) / groups;
+  return (unsigned)(g < 1 ? 1 : (g > cap ? cap : g));
+}
+
+// (waves per row, pieces per lane) for a row of D: one wave up to four pieces a lane, then a workgroup of 4 or 16
+struct RnShape { int wpr, nv; };
+RnShape rn_shape(int64_t D, int vec) {
+  if (D < vec) return {0, 0};                       // SMALL
+  const int64_t vecs = (D + vec - 1) / vec;
+  for (int wpr : {1, 4, 16})
+    for (int nv : {1, 2, 4})
+      if (vecs <= 64ll * wpr * nv) return {wpr, nv};
+  return {16, 8};
+}
+
+// RUN(pieces, waves per row, waves per workgroup, SMALL)
+#define RN_PICK(RUN)                                     \
+  switch (sh.wpr * 16 + sh.nv) {                         \
+    case 0: RUN(1, 1, 4, true); break;                   \
+    case 1 * 16 + 1: RUN(1, 1, 4, false); break;         \
+    case 1 * 16 + 2: RUN(2, 1, 4, false); break;         \
+    case 1 * 16 + 4: RUN(4, 1, 4, false); break;         \
+    case 4 * 16 + 1: RUN(1, 4, 4, false); break;         \
+    case 4 * 16 + 2: RUN(2, 4, 4, false); break;         \
+    case 4 * 16 + 4: RUN(4, 4, 4, false); break;         \
+    case 16 * 16 + 1: RUN(1, 16, 16, false); break;      \
+    case 16 * 16 + 2: RUN(2, 16, 16, false); break;      \
+    case 16 * 16 + 4: RUN(4, 16, 16, false); break;      \
+    default: RUN(8, 16, 16, false); break;               \
+  }
+
+template <class T, int MODE>
+int rn_launch_fwd(const RnFwd<T>& a, hipStream_t st) {
+  const RnShape sh = rn_shape(a.D, Elem<T>::VEC);
+  const unsigned grid = rn_grid(a.R, sh.wpr <= 1 ? 4 : 1, 8192);
+#define RN_F(NV, WPR, WAVES, SMALL) \
+  hipLaunchKernelGGL((k_rmsnorm_fwd<T, MODE, NV, WPR, WAVES, SMALL>), dim3(grid), dim3(64 * WAVES), 0, st, a)
+  RN_PICK(RN_F)
+#undef RN_F
+  return hotk_launch_status();
+}
+
+unsigned rn_bwd_grid(int64_t R, int wpr) { return rn_grid(R, wpr <= 1 ? 4 : 1, 1024); }
+
+template <class T>
+int rn_launch_bwd(const RnBwd<T>& a, hipStream_t st) {
+  const RnShape sh = rn_shape(a.D, Elem<T>::VEC);
+  const unsigned grid = rn_bwd_grid(a.R, sh.wpr);
+#define RN_B(NV, WPR, WAVES, SMALL) \
+  hipLaunchKernelGGL((k_rmsnorm_bwd<T, NV, WPR, WAVES, SMALL>), dim3(grid), dim3(64 * WAVES), 0, st, a)
+  RN_PICK(RN_B)
+#undef RN_B
+  return hotk_launch_status();
+}
+
+bool rn_rows_ok(const void* p, int64_t ld, int64_t D, int type) { return p && ld >= D && ffn_elem_aligned(p, type); }
+
+}  // namespace
+
+extern "C" int hotk_rmsnorm_supported(int64_t D, int type) { return (D > 0 && D <= RN_MAX_D && ffn_type_ok(type)) ? 1 : 0; }
+
+extern "C" int hotk_rmsnorm_fwd(const void* x, int64_t ld_x, const void* res, int64_t ld_res, const void* w, const uint8_t* kind,
+                                unsigned keep, float eps, void* y, void* h, float* rstd, int64_t R, int64_t D, int type,
+                                void* stream) {
+  HOTK_CHECK_ARG(R >= 0);
+  if (!hotk_rmsnorm_supported(D, type)) return HOTK_EUNSUPPORTED;
+  if (R == 0) return HOTK_OK;
+  HOTK_CHECK_ARG(rn_rows_ok(x, ld_x, D, type) && rn_rows_ok(w, D, D, type) && rn_rows_ok(y, D, D, type));
+  HOTK_CHECK_ARG(!res || (rn_rows_ok(res, ld_res, D, type) && rn_rows_ok(h, D, D, type)));
+  int rc = HOTK_OK;
+  ffn_dispatch(type, [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    const RnFwd<T> a{(const T*)x, (const T*)res, (const T*)w, ld_x, ld_res, kind, keep, eps, (T*)y, (T*)h, rstd, nullptr,
+                     nullptr, R, (int)D};
+    rc = rn_launch_fwd<T, RN_NORM>(a, (hipStream_t)stream);
+  });
+  return rc;
+}
+
+extern "C" int hotk_rmsnorm_quant(const void* x, int64_t ld_x, const void* res, int64_t ld_res, const void* w,
+                                  const uint8_t* kind, unsigned keep, float eps, uint8_t* q, float* scale, void* h, int64_t R,
+                                  int64_t D, int type, void* stream) {
+  HOTK_CHECK_ARG(R >= 0);
+  if (!hotk_rmsnorm_supported(D, type)) return HOTK_EUNSUPPORTED;
+  if (R == 0) return HOTK_OK;
+  HOTK_CHECK_ARG(rn_rows_ok(x, ld_x, D, type) && rn_rows_ok(w, D, D, type) && q && scale);
+  HOTK_CHECK_ARG(!res || (rn_rows_ok(res, ld_res, D, type) && rn_rows_ok(h, D, D, type)));
+  int rc = HOTK_OK;
+  ffn_dispatch(type, [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    const RnFwd<T> a{(const T*)x, (const T*)res, (const T*)w, ld_x, ld_res, kind, keep, eps, nullptr, (T*)h, nullptr, q,
+                     scale, R, (int)D};
+    rc = rn_launch_fwd<T, RN_NORM8>(a, (hipStream_t)stream);
+  });
+  return rc;
+}
+
+extern "C" int hotk_quantize_rows(const void* x, int64_t ld_x, uint8_t* q, float* scale, int64_t R, int64_t D, int type,
+                                  void* stream) {
+  HOTK_CHECK_ARG(R >= 0);
+  if (!hotk_rmsnorm_supported(D, type)) return HOTK_EUNSUPPORTED;
+  if (R == 0) return HOTK_OK;
+  HOTK_CHECK_ARG(rn_rows_ok(x, ld_x, D, type) && q && scale);
+  int rc = HOTK_OK;
+  ffn_dispatch(type, [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    const RnFwd<T> a{(const T*)x, nullptr, nullptr, ld_x, 0, nullptr, 0, 0.f, nullptr, nullptr, nullptr, q, scale, R, (int)D};
+    rc = rn_launch_fwd<T, RN_QUANT>(a, (hipStream_t)stream);
+  });
+  return rc;
+}
+
+extern "C" int hotk_rmsnorm_partials(int64_t R, int64_t D, int type, int64_t* n_partials) {
+  HOTK_CHECK_ARG(n_partials && R >= 0);
+  if (!hotk_rmsnorm_supported(D, type)) return HOTK_EUNSUPPORTED;
+  *n_partials = (int64_t)rn_bwd_grid(R, rn_shape(D, 16 / ffn_bytes(type)).wpr);
+  return HOTK_OK;
+}
+
+extern "C" int hotk_rmsnorm_bwd(const void* dy, int64_t ld_dy, const void* dh, int64_t ld_dh, const void* h, int64_t ld_h,
+                                const float* rstd, const void* w, const uint8_t* kind, unsigned keep, void* dx, float* partial,
+                                int64_t R, int64_t D, int type, void* stream) {
+  HOTK_CHECK_ARG(R >= 0);
+  if (!hotk_rmsnorm_supported(D, type)) return HOTK_EUNSUPPORTED;
+  HOTK_CHECK_ARG(partial);
+  HOTK_CHECK_ARG(R == 0 || (rn_rows_ok(dy, ld_dy, D, type) && rn_rows_ok(h, ld_h, D, type) && rstd && rn_rows_ok(dx, D, D, type)));
+  HOTK_CHECK_ARG(rn_rows_ok(w, D, D, type) && (!dh || rn_rows_ok(dh, ld_dh, D, type)));
+  int rc = HOTK_OK;
+  ffn_dispatch(type, [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    const RnBwd<T> a{(const T*)dy, (const T*)dh, (const T*)h, (const T*)w, ld_dy, ld_dh, ld_h, rstd, kind, keep, (T*)dx, partial,
+                     R, (int)D};
+    rc = rn_launch_bwd<T>(a, (hipStream_t)stream);
+  });
+  return rc;
+}
+
+extern "C" int hotk_sum_partials(const float* partial, int64_t n, int64_t D, void* out, int type, void* stream) {
+  HOTK_CHECK_ARG(n >= 0 && D >= 0);
+  if (!ffn_type_ok(type)) return HOTK_EUNSUPPORTED;
+  if (D == 0) return HOTK_OK;
+  HOTK_CHECK_ARG(out && (partial || n == 0) && ffn_elem_aligned(out, type));
+  const dim3 grid((unsigned)((D + 63) / 64)), block(64 * SP_WAVES);
+  ffn_dispatch(type, [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    hipLaunchKernelGGL(k_sum_partials<T>, grid, block, 0, (hipStream_t)stream, partial, n, D, (T*)out);
+  });
+  return hotk_launch_status();
+}

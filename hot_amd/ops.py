@@ -13,6 +13,7 @@ from torch.autograd import Function
 from . import _lib
 from ._lib import lib, p, check, call, stream_ptr, rows2d, KEEP_DIAG, KEEP_OFFDIAG, KEEP_VALID, SEG_CHUNK
 from .plan import Seg
+from .ffn import rms_norm, rms_norm_quantized, quantize_rows, linear_act, linear_act_quantized  # noqa: F401
 
 
 # ------------------------------------------------------------------------------------------------

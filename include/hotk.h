@@ -501,6 +501,65 @@ enum { HOTK_ATTN22_FWD_GRAPHSUM = 0, HOTK_ATTN22_FWD_NODESUM = 1, HOTK_ATTN22_FW
        HOTK_ATTN22_BWD_KEYVAL_GRAPH = 7, HOTK_ATTN22_BWD_KEYVAL_NODE = 8 };
 int hotk_attn22_phase(const hotk_attn22_args* args, int phase, void* workspace, size_t ws_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * The feed-forward block of a pre-norm layer as operators: root-mean-square norm of a residual stream, rows to 8 bits,
+ * matrix product with bias, activation and residual in its epilogue.  `type` is the element type of every void* tensor
+ * that names none of its own; `ld*` counts elements; rows may start at any element.  Outputs without an `ld` are
+ * contiguous.  Sums, statistics and epilogues are in 32 bits, results are rounded once.
+ * ---------------------------------------------------------------------------------------------- */
+#define HOTK_F32 0
+#define HOTK_BF16 1
+#define HOTK_F16 2
+#define HOTK_E4M3 3          /* OCP e4m3 (finite, largest 448), operands of hotk_linear_act only */
+
+/* h[r] = x[r] + res[r] (rounded to the type; res NULL: h = x, and h is not written), rstd[r] = (mean h^2 + eps)^-1/2 (NULL: not
+ * written), y[r] = h[r] rstd[r] w.  Rows that `keep` leaves out (kind NULL: none) are not read; their y and h are zero.
+ * 0 < D <= 32768 (hotk_rmsnorm_supported). */
+int hotk_rmsnorm_supported(int64_t D, int type);
+int hotk_rmsnorm_fwd(const void* x, int64_t ld_x, const void* res, int64_t ld_res, const void* w, const uint8_t* kind,
+                     unsigned keep, float eps, void* y, void* h, float* rstd, int64_t R, int64_t D, int type, void* stream);
+/* the same norm with an 8-bit result: scale[r] = max(max_c |y| / 448, 2^-126), q[r] = e4m3(y / scale[r]), y in 32 bits.  A row
+ * that holds an infinity or NaN has a scale that is one. */
+int hotk_rmsnorm_quant(const void* x, int64_t ld_x, const void* res, int64_t ld_res, const void* w, const uint8_t* kind,
+                       unsigned keep, float eps, uint8_t* q, float* scale, void* h, int64_t R, int64_t D, int type,
+                       void* stream);
+/* rows of x to 8 bits with one scale each, as above */
+int hotk_quantize_rows(const void* x, int64_t ld_x, uint8_t* q, float* scale, int64_t R, int64_t D, int type, void* stream);
+/* dx[r] (the gradient of x and of res) from dy, the gradient dh of h (NULL: none), h and rstd; partial[n][D], n =
+ * hotk_rmsnorm_partials(R, D, type): dw's partial sums, added up in order by hotk_sum_partials */
+int hotk_rmsnorm_partials(int64_t R, int64_t D, int type, int64_t* n_partials);
+int hotk_rmsnorm_bwd(const void* dy, int64_t ld_dy, const void* dh, int64_t ld_dh, const void* h, int64_t ld_h,
+                     const float* rstd, const void* w, const uint8_t* kind, unsigned keep, void* dx, float* partial, int64_t R,
+                     int64_t D, int type, void* stream);
+/* out[c] = sum over b < n of partial[b][c], rounded to the type; the order of the sum goes by n and D alone */
+int hotk_sum_partials(const float* partial, int64_t n, int64_t D, void* out, int type, void* stream);
+
+/* y = act(z) + res, z = x w^T + bias; x [M, K], w [N, K] (the layout of torch.nn.Linear).  type HOTK_E4M3: z = x_scale[m]
+ * w_scale[n] (x w^T) + bias, with bias, res and y in out_type; otherwise out_type = type.  save (NULL: none) [M, N]: what
+ * hotk_linear_turn needs for the gradient, int16 for 16-bit types, fp32 for HOTK_F32; not written for HOTK_ACT_NONE.
+ * Rows of x and w: whole, aligned 16-byte pieces (K, ld_x, ld_w times the element size, and both pointers; else
+ * HOTK_EUNSUPPORTED: hotk_linear_turn makes padded copies). */
+enum { HOTK_ACT_NONE = 0, HOTK_ACT_RELU = 1, HOTK_ACT_LEAKYRELU = 2 /* slope 0.01 */, HOTK_ACT_GELU = 3 /* exact, by erf */,
+       HOTK_ACT_TANH = 4, HOTK_ACT_SILU = 5 };
+typedef struct {
+  int64_t M, N, K;
+  const void* x; int64_t ld_x;
+  const void* w; int64_t ld_w;
+  const void* bias;
+  const void* res; int64_t ld_res;
+  void* y; int64_t ld_y;
+  void* save;
+  const float* x_scale;
+  const float* w_scale;
+  int32_t type, out_type, act, reserved;
+} hotk_linear_args;
+int hotk_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int type, size_t* bytes);
+int hotk_linear_act(const hotk_linear_args* args, void* workspace, size_t ws_bytes, void* stream);
+/* v = in [R, C] times the slope that `save` holds (HOTK_ACT_NONE: times one); out [R, ld_out] and out_t [C, ld_t] (its transpose),
+ * each NULL or written with zeros up to its row length; partial (NULL: none) [ceil(R / 64)][C]: column sums of v */
+int hotk_linear_turn(const void* in, int64_t ld_in, const void* save, int act, void* out, int64_t ld_out, void* out_t,
+                     int64_t ld_t, float* partial, int64_t R, int64_t C, int type, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
