@@ -123,9 +123,6 @@ class LinearArgs(ctypes.Structure):
                 ('type', ctypes.c_int32), ('out_type', ctypes.c_int32), ('act', ctypes.c_int32), ('reserved', ctypes.c_int32)]
 
 
-TYPE_F32, TYPE_BF16, TYPE_F16, TYPE_E4M3 = range(4)
-ACTS = {'none': 0, 'relu': 1, 'leakyrelu': 2, 'gelu': 3, 'tanh': 4, 'silu': 5}
-
 _SIGNATURES.update({
     'hotk_rmsnorm_supported': [_L, _I],
     'hotk_rmsnorm_fwd': [_P, _L, _P, _L, _P, _P, _U, _F, _P, _P, _P, _L, _L, _I, _P],
@@ -167,6 +164,21 @@ def lib():
     return _lib
 
 
+def torch_binding():
+    """the compiled host side of the feed-forward operators (csrc/ffn_torch.cpp), tied to the library that lib() loaded"""
+    L = lib()
+    try:
+        from . import _ffn
+    except ImportError as e:
+        raise HotkError(f'hot_amd/_ffn is missing or does not load ({e}): build it with `python -m hot_amd.build`') from None
+    _ffn.bind({n: ctypes.cast(getattr(L, n), c_void_p).value for n in EXPORTS if n.startswith(('hotk_rmsnorm', 'hotk_quantize', 'hotk_sum_partials', 'hotk_linear_', 'hotk_strerror'))},
+              HotkError)
+    _ffn.set_timing(_timing_hook if _timing is not None else None)
+    global _ffn_module
+    _ffn_module = _ffn
+    return _ffn
+
+
 def check(rc, what):
     if rc != 0:
         raise HotkError(f'{what} failed: {lib().hotk_strerror(rc).decode()} ({rc})')
@@ -176,18 +188,36 @@ def check(rc, what):
 # optional live timing of C-ABI launches with HIP events on the launch stream (used by bench.py)
 # ------------------------------------------------------------------------------------------------
 _timing = None   # None = off; else {'only': name or None, 'events': [(name, start, end, alg_bytes)]}
+_ffn_module = None
+
+
+def _timing_hook(name, alg_bytes, before):
+    """what call() does around a launch, for the launches of csrc/ffn_torch.cpp"""
+    t = _timing
+    if t is None or (t['only'] is not None and t['only'] != name):
+        return
+    e = torch.cuda.Event(enable_timing=True)
+    e.record()
+    if before:
+        t['begun'] = e
+    elif 'begun' in t:
+        t['events'].append((name, t.pop('begun'), e, int(alg_bytes)))
 
 
 def timing_begin(only=None):
     """Record a HIP event pair around every launch of `only` (or of every entry point when None)."""
     global _timing
     _timing = {'only': only, 'events': []}
+    if _ffn_module is not None:
+        _ffn_module.set_timing(_timing_hook)
 
 
 def timing_end():
     """-> {entry point: (total ms, launches, algorithmic bytes)}; synchronises the device."""
     global _timing
     t, _timing = _timing, None
+    if _ffn_module is not None:
+        _ffn_module.set_timing(None)
     out = {}
     if not t:
         return out

@@ -1,4 +1,4 @@
-"""Build libhotk.so in-tree with hipcc for gfx950 (`python -m hot_amd.build`).
+"""Build libhotk.so in-tree with hipcc for gfx950, and hot_amd/_ffn beside it (`python -m hot_amd.build`).
 
 One object per csrc/*.hip (compiled in parallel, only when the source or a header is newer), linked into
 hot_amd/libhotk.so.  Objects live under hot_amd/csrc/_obj/ (git-ignored)."""
@@ -8,6 +8,7 @@ import os
 import re
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -74,6 +75,31 @@ def build(force=False, verbose=True, extra_flags=(), out=OUT):
     return out
 
 
+EXT_SRC = os.path.join(HERE, 'csrc', 'ffn_torch.cpp')
+EXT_OUT = os.path.join(HERE, '_ffn' + sysconfig.get_config_var('EXT_SUFFIX'))
+
+
+def build_ext(force=False, verbose=True):
+    """hot_amd/_ffn: the compiled host side of the feed-forward operators (torch's C++ interface; host code only).  It takes
+    libhotk's entries from the running process, so it is linked against torch alone."""
+    import torch
+    from torch.utils import cpp_extension
+    newest = max(os.path.getmtime(f) for f in (EXT_SRC, os.path.join(HERE, '..', 'include', 'hotk.h')))
+    if not force and os.path.exists(EXT_OUT) and os.path.getmtime(EXT_OUT) >= newest:
+        return EXT_OUT
+    lib = os.path.join(os.path.dirname(torch.__file__), 'lib')
+    cmd = ['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-w', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
+           f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}']
+    for d in cpp_extension.include_paths(device_type='cuda') + [sysconfig.get_paths()['include']]:
+        cmd += ['-isystem', d]
+    cmd += [EXT_SRC, '-o', EXT_OUT, '-L' + lib, '-Wl,-rpath,' + lib, '-lc10', '-lc10_hip', '-ltorch', '-ltorch_cpu', '-ltorch_hip',
+            '-ltorch_python']
+    if verbose:
+        print(' '.join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return EXT_OUT
+
+
 def assembly(src, out, extra_flags=()):
     """device assembly of one source, compiled with the library's own flags (for tests/asm_hazards.py)"""
     hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
@@ -84,3 +110,4 @@ def assembly(src, out, extra_flags=()):
 
 if __name__ == '__main__':
     build(force='--force' in sys.argv)
+    build_ext(force='--force' in sys.argv)

@@ -1,0 +1,495 @@
+// Host side of the feed-forward operators (hot_amd/ffn.py): argument checks, result and workspace tensors, autograd nodes, and the
+// launches through the C entries of libhotk.so.  In C++ because a call is a few microseconds of GPU work at the small end: the
+// same steps in Python (ctypes arguments, a Python autograd function) cost 16 us a forward call and 160 us a call with its
+// gradients, against 5 and 25 here.
+//
+// The entries' addresses come from Python's loaded library (bind), so both bindings run the same build of it; with timing on
+// (_lib.timing_begin) every launch is reported to the same hook as Python's own.
+#include <ATen/ATen.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/python.h>
+
+#include <atomic>
+#include <optional>
+#include <stdexcept>
+#include <string>
+
+#include "../../include/hotk.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using std::optional;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace {
+
+struct Refused : std::runtime_error {      // becomes hot_amd._lib.HotkError
+  using std::runtime_error::runtime_error;
+};
+PyObject* error_type = nullptr;
+
+template <class... A>
+[[noreturn]] void refuse(const A&... parts) {
+  throw Refused(c10::str(parts...));
+}
+
+// ---- the library -------------------------------------------------------------------------------------------------------
+struct Entries {
+  decltype(&hotk_strerror) strerror;
+  decltype(&hotk_rmsnorm_supported) rmsnorm_supported;
+  decltype(&hotk_rmsnorm_fwd) rmsnorm_fwd;
+  decltype(&hotk_rmsnorm_quant) rmsnorm_quant;
+  decltype(&hotk_quantize_rows) quantize_rows;
+  decltype(&hotk_rmsnorm_partials) rmsnorm_partials;
+  decltype(&hotk_rmsnorm_bwd) rmsnorm_bwd;
+  decltype(&hotk_sum_partials) sum_partials;
+  decltype(&hotk_linear_workspace_bytes) linear_workspace_bytes;
+  decltype(&hotk_linear_act) linear_act;
+  decltype(&hotk_linear_turn) linear_turn;
+} L{};
+
+template <class F>
+void bind_one(F& f, const py::dict& d, const char* name) {
+  f = reinterpret_cast<F>(d[name].cast<uintptr_t>());
+}
+
+void bind(const py::dict& d, py::object error) {
+  bind_one(L.strerror, d, "hotk_strerror");
+  bind_one(L.rmsnorm_supported, d, "hotk_rmsnorm_supported");
+  bind_one(L.rmsnorm_fwd, d, "hotk_rmsnorm_fwd");
+  bind_one(L.rmsnorm_quant, d, "hotk_rmsnorm_quant");
+  bind_one(L.quantize_rows, d, "hotk_quantize_rows");
+  bind_one(L.rmsnorm_partials, d, "hotk_rmsnorm_partials");
+  bind_one(L.rmsnorm_bwd, d, "hotk_rmsnorm_bwd");
+  bind_one(L.sum_partials, d, "hotk_sum_partials");
+  bind_one(L.linear_workspace_bytes, d, "hotk_linear_workspace_bytes");
+  bind_one(L.linear_act, d, "hotk_linear_act");
+  bind_one(L.linear_turn, d, "hotk_linear_turn");
+  error_type = error.release().ptr();      // kept for the process
+}
+
+void check(int rc, const char* what) {
+  if (rc != HOTK_OK) refuse(what, " failed: ", L.strerror(rc), " (", rc, ")");
+}
+
+// the timing hook: called with (name, bytes, True) before and (name, bytes, False) after a launch while it is set
+std::atomic<bool> timing{false};
+PyObject* timing_hook = nullptr;           // touched under the GIL only
+
+void set_timing(py::object hook) {
+  Py_XDECREF(timing_hook);
+  timing_hook = hook.is_none() ? nullptr : hook.release().ptr();
+  timing = timing_hook != nullptr;
+}
+
+template <class F>
+void launch(const char* name, int64_t bytes, F&& f) {
+  int rc;
+  if (timing.load(std::memory_order_relaxed)) {
+    py::gil_scoped_acquire gil;
+    py::object hook = timing_hook ? py::reinterpret_borrow<py::object>(timing_hook) : py::none();
+    if (!hook.is_none()) hook(name, bytes, true);
+    rc = f();
+    if (!hook.is_none()) hook(name, bytes, false);
+  } else {
+    rc = f();
+  }
+  check(rc, name);
+}
+
+// ---- arguments ---------------------------------------------------------------------------------------------------------
+int type_of(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat: return HOTK_F32;
+    case at::kBFloat16: return HOTK_BF16;
+    case at::kHalf: return HOTK_F16;
+    case at::kFloat8_e4m3fn: return HOTK_E4M3;
+    default: return -1;
+  }
+}
+
+void check_input(const Tensor& x, const char* what, bool eight = false) {
+  if (!x.defined()) refuse(what, ": a tensor is expected");
+  if (!x.is_cuda())
+    refuse("hot_amd kernels run on a HIP device only; ", what, " is on ", x.device(), ". There is no CPU path: move it to the GPU.");
+  const int ty = type_of(x.scalar_type());
+  if (eight ? ty != HOTK_E4M3 : (ty < 0 || ty == HOTK_E4M3))
+    refuse(what, ": ", eight ? "float8_e4m3fn" : "fp32, bf16 or fp16", " expected, got ", x.scalar_type());
+  if (x.layout() != at::kStrided) refuse(what, ": a strided tensor is expected");
+  if (x.dim() < 1 || x.size(-1) == 0) refuse(what, ": [..., width] with width >= 1 expected, got shape ", x.sizes());
+}
+
+// an operand that goes with `ref`: on its device, of this type and shape
+void check_with(const Tensor& ref, const Tensor& t, const char* what, at::IntArrayRef shape, at::ScalarType type) {
+  if (!t.defined()) refuse(what, ": a tensor is expected");
+  if (t.device() != ref.device()) refuse(what, " is on ", t.device(), ", the input on ", ref.device());
+  if (t.scalar_type() != type) refuse(what, ": ", type, " expected, got ", t.scalar_type());
+  if (t.layout() != at::kStrided) refuse(what, ": a strided tensor is expected");
+  if (t.sizes() != shape) refuse(what, ": shape ", shape, " expected, got ", t.sizes());
+}
+
+// [..., C] as rows in place: the tensor, elements from row to row, rows; a copy where the rows lie at no single stride
+struct Rows {
+  Tensor t;
+  int64_t ld = 0, n = 0;
+  const void* p() const { return t.defined() ? t.const_data_ptr() : nullptr; }
+};
+
+Rows rows(const Tensor& x) {
+  const int64_t C = x.size(-1), n = x.numel() / C;
+  if (n == 0) return {x, C, 0};
+  if (x.stride(-1) == 1 || C == 1) {
+    int64_t ld = -1, span = 1;             // span: rows that the dimensions to the right hold
+    bool ok = true;
+    for (int64_t k = x.dim() - 2; k >= 0 && ok; --k) {
+      if (x.size(k) != 1) {
+        if (ld < 0) ld = x.stride(k);      // the innermost dimension of more than one
+        ok = x.stride(k) == ld * span;
+      }
+      span *= x.size(k);
+    }
+    if (ld < 0) ld = C;
+    if (ok && ld >= C) return {x, ld, n};
+  }
+  return {x.contiguous(), C, n};
+}
+Rows rows(const optional<Tensor>& x) { return x ? rows(*x) : Rows{}; }
+
+void* stream_of(const Tensor& x) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index()).stream(); }
+Tensor like(const Tensor& x, at::IntArrayRef shape, at::ScalarType type) { return at::empty(shape, x.options().dtype(type)); }
+Tensor like(const Tensor& x) { return like(x, x.sizes(), x.scalar_type()); }
+void* out(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+bool wants_grad(const optional<Tensor>& t) { return t && wants_grad(*t); }
+template <class... T>
+void refuse_grad(const char* what, const T&... t) {
+  if (at::GradMode::is_enabled() && (wants_grad(t) || ...))
+    refuse(what, " has no gradient: call it under torch.no_grad() or on detached tensors");
+}
+void first_order(const char* what) {
+  if (at::GradMode::is_enabled()) refuse(what, " has gradients of first order only (create_graph=True asks for more)");
+}
+
+// ---- norm --------------------------------------------------------------------------------------------------------------
+void check_norm(const Tensor& x, const Tensor& w, const optional<Tensor>& r, const optional<Tensor>& kind, int64_t keep, double eps) {
+  check_input(x, "x");
+  const int64_t D = x.size(-1);
+  check_with(x, w, "weight", {D}, x.scalar_type());
+  if (r) check_with(x, *r, "residual", x.sizes(), x.scalar_type());
+  if (L.rmsnorm_supported(D, type_of(x.scalar_type())) != 1) refuse("rows of up to 32768 elements are normalised, got ", D);
+  if (keep < 0 || keep > 0xffffffffll) refuse("keep: a bit set over kinds expected, got ", keep);
+  if (!(eps >= 0.)) refuse("eps: a number >= 0 expected, got ", eps);
+  if (kind && (!kind->defined() || kind->scalar_type() != at::kByte || kind->numel() != x.numel() / D || kind->device() != x.device()))
+    refuse("kind: uint8, one per row (", x.numel() / D, "), on ", x.device(), " expected");
+}
+Tensor kind_of(const optional<Tensor>& kind) { return kind ? kind->contiguous() : Tensor(); }
+const uint8_t* kind_ptr(const Tensor& k) { return k.defined() ? k.const_data_ptr<uint8_t>() : nullptr; }
+
+// y (and h), and what the backward pass needs
+struct Normed {
+  Tensor y, h, rstd, w, kind;
+};
+Normed norm_forward(const Tensor& x, const Tensor& weight, const optional<Tensor>& r, const optional<Tensor>& kind, int64_t keep,
+                    double eps, bool grad) {
+  const c10::DeviceGuard guard(x.device());
+  const int64_t D = x.size(-1);
+  const Rows xs = rows(x), rs = rows(r);
+  Normed o;
+  o.w = weight.contiguous();
+  o.kind = kind_of(kind);
+  o.y = like(x);
+  if (r) o.h = like(x);
+  if (grad) o.rstd = like(x, {xs.n}, at::kFloat);
+  if (xs.n)
+    launch("hotk_rmsnorm_fwd", (r ? 4 : 2) * x.numel() * x.element_size(), [&] {
+      return L.rmsnorm_fwd(xs.p(), xs.ld, rs.p(), rs.ld, o.w.const_data_ptr(), kind_ptr(o.kind), (unsigned)keep, (float)eps, o.y.data_ptr(),
+                           out(o.h), (float*)out(o.rstd), xs.n, D, type_of(x.scalar_type()), stream_of(x));
+    });
+  return o;
+}
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const optional<Tensor>& r,
+                               const optional<Tensor>& kind, int64_t keep, double eps) {
+    ctx->set_materialize_grads(false);
+    Normed o = norm_forward(x, weight, r, kind, keep, eps, true);
+    ctx->save_for_backward({r ? o.h : x, o.rstd, o.w, o.kind});
+    ctx->saved_data["keep"] = keep;
+    ctx->saved_data["wants"] = (int64_t)(wants_grad(x) | wants_grad(weight) << 1 | wants_grad(r) << 2 | (r ? 1 : 0) << 3);
+    if (r) return {o.y, o.h};
+    return {o.y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    first_order("rms_norm");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &h = saved[0], &rstd = saved[1], &w = saved[2], &kind = saved[3];
+    const int64_t wants = ctx->saved_data["wants"].toInt(), keep = ctx->saved_data["keep"].toInt();
+    const bool has_r = wants & 8;
+    Tensor dy = g[0], dh = has_r ? g[1] : Tensor(), dx, dw;
+    if (dy.defined() || dh.defined()) {
+      const c10::DeviceGuard guard(h.device());
+      const int ty = type_of(h.scalar_type());
+      const int64_t D = h.size(-1);
+      if (!dy.defined()) dy = at::zeros_like(h);
+      const Rows hs = rows(h), gs = rows(dy), ss = dh.defined() ? rows(dh) : Rows{};
+      void* st = stream_of(h);
+      int64_t parts = 0;
+      check(L.rmsnorm_partials(hs.n, D, ty, &parts), "hotk_rmsnorm_partials");
+      dx = like(h);
+      const Tensor part = like(h, {parts, D}, at::kFloat);
+      launch("hotk_rmsnorm_bwd", (dh.defined() ? 4 : 3) * h.numel() * h.element_size(), [&] {
+        return L.rmsnorm_bwd(gs.p(), gs.ld, ss.p(), ss.ld, hs.p(), hs.ld, rstd.const_data_ptr<float>(), w.const_data_ptr(), kind_ptr(kind),
+                             (unsigned)keep, dx.data_ptr(), part.data_ptr<float>(), hs.n, D, ty, st);
+      });
+      if (wants & 2) {
+        dw = like(h, {D}, h.scalar_type());
+        launch("hotk_sum_partials", 4 * parts * D, [&] { return L.sum_partials(part.const_data_ptr<float>(), parts, D, dw.data_ptr(), ty, st); });
+      }
+    }
+    return {wants & 1 ? dx : Tensor(), dw, wants & 4 ? dx : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+py::object rms_norm(const Tensor& x, const Tensor& weight, const optional<Tensor>& r, double eps, const optional<Tensor>& kind, int64_t keep) {
+  check_norm(x, weight, r, kind, keep, eps);
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(r))) {
+    const variable_list o = RmsNorm::apply(x, weight, r, kind, keep, eps);
+    return r ? py::object(py::make_tuple(o[0], o[1])) : py::cast(o[0]);
+  }
+  const Normed o = norm_forward(x, weight, r, kind, keep, eps, false);
+  return r ? py::object(py::make_tuple(o.y, o.h)) : py::cast(o.y);
+}
+
+py::tuple rms_norm_quantized(const Tensor& x, const Tensor& weight, const optional<Tensor>& r, double eps, const optional<Tensor>& kind,
+                             int64_t keep) {
+  check_norm(x, weight, r, kind, keep, eps);
+  refuse_grad("rms_norm_quantized", x, weight, r);
+  const c10::DeviceGuard guard(x.device());
+  const int64_t D = x.size(-1);
+  const Rows xs = rows(x), rs = rows(r);
+  const Tensor w = weight.contiguous(), k = kind_of(kind), q = like(x, x.sizes(), at::kFloat8_e4m3fn);
+  const Tensor scale = like(x, x.sizes().slice(0, x.dim() - 1), at::kFloat), h = r ? like(x) : Tensor();
+  if (xs.n)
+    launch("hotk_rmsnorm_quant", x.numel() * (1 + (r ? 3 : 1) * x.element_size()), [&] {
+      return L.rmsnorm_quant(xs.p(), xs.ld, rs.p(), rs.ld, w.const_data_ptr(), kind_ptr(k), (unsigned)keep, (float)eps, (uint8_t*)q.data_ptr(),
+                             scale.data_ptr<float>(), out(h), xs.n, D, type_of(x.scalar_type()), stream_of(x));
+    });
+  return r ? py::make_tuple(q, scale, h) : py::make_tuple(q, scale);
+}
+
+py::tuple quantize_rows(const Tensor& x) {
+  check_input(x, "x");
+  refuse_grad("quantize_rows", x);
+  const int64_t D = x.size(-1);
+  const int ty = type_of(x.scalar_type());
+  if (L.rmsnorm_supported(D, ty) != 1) refuse("rows of up to 32768 elements are quantized, got ", D);
+  const c10::DeviceGuard guard(x.device());
+  const Rows xs = rows(x);
+  const Tensor q = like(x, x.sizes(), at::kFloat8_e4m3fn), scale = like(x, x.sizes().slice(0, x.dim() - 1), at::kFloat);
+  if (xs.n)
+    launch("hotk_quantize_rows", x.numel() * (1 + x.element_size()), [&] {
+      return L.quantize_rows(xs.p(), xs.ld, (uint8_t*)q.data_ptr(), scale.data_ptr<float>(), xs.n, D, ty, stream_of(x));
+    });
+  return py::make_tuple(q, scale);
+}
+
+// ---- product -----------------------------------------------------------------------------------------------------------
+int64_t up(int64_t n, int64_t size) {      // n elements of `size` bytes in whole 16-byte pieces
+  const int64_t m = 16 / size;
+  return (n + m - 1) / m * m;
+}
+bool whole(const Rows& x, int64_t C) {     // rows as the product reads them: whole, aligned 16-byte pieces
+  const int64_t e = x.t.element_size();
+  return C * e % 16 == 0 && x.ld * e % 16 == 0 && (uintptr_t)x.p() % 16 == 0;
+}
+
+// v = in * slope -> any of out [R, ld_out], out_t [C, ld_t], column sums by 64 rows
+void turn(const Rows& in, int64_t C, const Tensor& save, int act, const Tensor& o, int64_t ld_o, const Tensor& o_t, int64_t ld_t,
+          const Tensor& part) {
+  launch("hotk_linear_turn", in.n * C * in.t.element_size() * (1 + o.defined() + o_t.defined()), [&] {
+    return L.linear_turn(in.p(), in.ld, out(save), act, out(o), ld_o, out(o_t), ld_t, (float*)out(part), in.n, C, type_of(in.t.scalar_type()),
+                         stream_of(in.t));
+  });
+}
+Rows turned(const Rows& in, int64_t C) {   // the transpose, rows of n padded with zeros to whole pieces
+  const int64_t ld = up(in.n, in.t.element_size());
+  const Tensor o = like(in.t, {C, ld}, in.t.scalar_type());
+  turn(in, C, {}, HOTK_ACT_NONE, {}, 0, o, ld, {});
+  return {o, ld, C};
+}
+Rows padded(const Rows& in, int64_t C) {   // itself where it is whole, else a copy with zeros behind each row
+  if (in.n == 0 || whole(in, C)) return in;
+  const int64_t ld = up(C, in.t.element_size());
+  const Tensor o = like(in.t, {in.n, ld}, in.t.scalar_type());
+  turn(in, C, {}, HOTK_ACT_NONE, o, ld, {}, 0, {});
+  return {o, ld, in.n};
+}
+
+struct Extras {
+  Tensor bias, save, x_scale, w_scale;
+  Rows res;
+  int act = HOTK_ACT_NONE;
+};
+// [x.n, w.n] = epilogue(x w^T); rows of K elements in whole pieces
+Tensor product(const Rows& x, const Rows& w, int64_t K, at::ScalarType type, const Extras& e) {
+  const int64_t M = x.n, N = w.n;
+  const Tensor y = like(x.t, {M, N}, type);
+  if (M == 0) return y;
+  const int ty = type_of(x.t.scalar_type());
+  size_t need = 0;
+  check(L.linear_workspace_bytes(M, N, K, ty, &need), "hotk_linear_workspace_bytes");
+  const Tensor ws = need ? like(x.t, {(int64_t)need}, at::kByte) : Tensor();
+  hotk_linear_args a{};
+  a.M = M; a.N = N; a.K = K;
+  a.x = x.p(); a.ld_x = x.ld;
+  a.w = w.p(); a.ld_w = w.ld;
+  a.bias = out(e.bias);
+  a.res = e.res.p(); a.ld_res = e.res.ld;
+  a.y = y.data_ptr(); a.ld_y = N;
+  a.save = out(e.save);
+  a.x_scale = (const float*)out(e.x_scale); a.w_scale = (const float*)out(e.w_scale);
+  a.type = ty; a.out_type = type_of(type); a.act = e.act;
+  launch("hotk_linear_act", (M + N) * K * x.t.element_size() + M * N * y.element_size() * (1 + e.res.t.defined()),
+         [&] { return L.linear_act(&a, out(ws), need, stream_of(x.t)); });
+  return y;
+}
+
+int act_code(const std::string& act) {
+  static const char* const names[] = {"none", "relu", "leakyrelu", "gelu", "tanh", "silu"};
+  for (int i = 0; i < 6; ++i)
+    if (act == names[i]) return i;
+  refuse("act: one of none, relu, leakyrelu, gelu, tanh, silu expected, got ", act);
+}
+
+std::vector<int64_t> result_shape(const Tensor& x, int64_t N) {
+  std::vector<int64_t> s(x.sizes().begin(), x.sizes().end());
+  s.back() = N;
+  return s;
+}
+
+void check_linear(const Tensor& x, const Tensor& w, const optional<Tensor>& b, const optional<Tensor>& r, at::ScalarType type) {
+  if (!w.defined() || w.dim() != 2 || w.size(0) == 0) refuse("weight: [N, K] with N >= 1 expected");
+  const int64_t N = w.size(0), K = w.size(1);
+  if (x.size(-1) != K) refuse("x has rows of ", x.size(-1), ", weight of ", K);
+  check_with(x, w, "weight", {N, K}, x.scalar_type());
+  if (b) check_with(x, *b, "bias", {N}, type);
+  if (r) check_with(x, *r, "residual", result_shape(x, N), type);
+}
+
+Tensor linear_forward(const Tensor& x, const Tensor& weight, const optional<Tensor>& b, const optional<Tensor>& r, int act, bool grad,
+                      Tensor* save) {
+  const c10::DeviceGuard guard(x.device());
+  const int64_t K = x.size(-1), N = weight.size(0);
+  const Rows xs = padded(rows(x), K), ws = padded(rows(weight), K);
+  Extras e;
+  e.act = act;
+  if (b) e.bias = b->contiguous();
+  e.res = rows(r);
+  if (grad && act) *save = e.save = like(x, {xs.n, N}, x.scalar_type() == at::kFloat ? at::kFloat : at::kShort);
+  return product(xs, ws, up(K, x.element_size()), x.scalar_type(), e).view(result_shape(x, N));
+}
+
+struct LinearAct : torch::autograd::Function<LinearAct> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const optional<Tensor>& b, const optional<Tensor>& r,
+                        int64_t act) {
+    ctx->set_materialize_grads(false);
+    Tensor save;
+    const bool inner = wants_grad(x) || wants_grad(weight) || wants_grad(b);
+    const Tensor y = linear_forward(x, weight, b, r, (int)act, inner, &save);
+    ctx->save_for_backward({x, weight, save});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["wants"] = (int64_t)(wants_grad(x) | wants_grad(weight) << 1 | wants_grad(b) << 2 | wants_grad(r) << 3);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    first_order("linear_act");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1], &save = saved[2], &dy = g[0];
+    const int act = (int)ctx->saved_data["act"].toInt();
+    const int64_t wants = ctx->saved_data["wants"].toInt(), K = x.size(-1), N = weight.size(0);
+    Tensor dx, dw, db;
+    if (dy.defined() && (wants & 7)) {
+      const c10::DeviceGuard guard(x.device());
+      const auto type = x.scalar_type();
+      const int64_t size = x.element_size(), M = x.numel() / K;
+      if (M == 0) {
+        if (wants & 1) dx = at::zeros_like(x);
+        if (wants & 2) dw = at::zeros_like(weight);
+        if (wants & 4) db = at::zeros({N}, x.options());
+      } else {
+        const Rows gs = rows(dy);
+        const int64_t Np = up(N, size), Mp = up(M, size);
+        // one pass over dy: dz where it is not dy itself, its transpose for dw, its column sums
+        const bool itself = act == HOTK_ACT_NONE && whole(gs, N);
+        const Tensor dz = wants & 1 && !itself ? like(x, {M, Np}, type) : Tensor();
+        const Tensor dzt = wants & 2 ? like(x, {N, Mp}, type) : Tensor();
+        const Tensor part = wants & 4 ? like(x, {(M + 63) / 64, N}, at::kFloat) : Tensor();
+        if (dz.defined() || dzt.defined() || part.defined()) turn(gs, N, save, act, dz, Np, dzt, Mp, part);
+        if (wants & 4) {
+          db = like(x, {N}, type);
+          launch("hotk_sum_partials", 4 * part.numel(), [&] {
+            return L.sum_partials(part.const_data_ptr<float>(), part.size(0), N, db.data_ptr(), type_of(type), stream_of(x));
+          });
+        }
+        if (wants & 1) dx = product(itself ? gs : Rows{dz, Np, M}, turned(rows(weight), K), Np, type, {}).view(x.sizes());
+        if (wants & 2) dw = product({dzt, Mp, N}, turned(rows(x), K), Mp, type, {});
+      }
+    }
+    return {dx, dw, db, wants & 8 ? dy : Tensor(), Tensor()};
+  }
+};
+
+Tensor linear_act(const Tensor& x, const Tensor& weight, const optional<Tensor>& b, const std::string& act, const optional<Tensor>& r) {
+  check_input(x, "x");
+  const int code = act_code(act);
+  check_linear(x, weight, b, r, x.scalar_type());
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(b) || wants_grad(r)))
+    return LinearAct::apply(x, weight, b, r, (int64_t)code);
+  Tensor none;
+  return linear_forward(x, weight, b, r, code, false, &none);
+}
+
+Tensor linear_act_quantized(const Tensor& xq, const Tensor& x_scale, const Tensor& wq, const Tensor& w_scale, const optional<Tensor>& b,
+                            const std::string& act, const optional<Tensor>& r, py::object out_dtype) {
+  check_input(xq, "xq", true);
+  if (!THPDtype_Check(out_dtype.ptr())) refuse("out_dtype: fp32, bf16 or fp16 expected");
+  const auto type = reinterpret_cast<THPDtype*>(out_dtype.ptr())->scalar_type;
+  if (type_of(type) < 0 || type_of(type) == HOTK_E4M3) refuse("out_dtype: fp32, bf16 or fp16 expected, got ", type);
+  const int code = act_code(act);
+  check_linear(xq, wq, b, r, type);
+  check_with(xq, x_scale, "x_scale", xq.sizes().slice(0, xq.dim() - 1), at::kFloat);
+  check_with(xq, w_scale, "w_scale", {wq.size(0)}, at::kFloat);
+  refuse_grad("linear_act_quantized", b, r, x_scale, w_scale);
+  const c10::DeviceGuard guard(xq.device());
+  const int64_t K = xq.size(-1);
+  Extras e;
+  e.act = code;
+  if (b) e.bias = b->contiguous();
+  e.res = rows(r);
+  e.x_scale = x_scale.contiguous();
+  e.w_scale = w_scale.contiguous();
+  return product(padded(rows(xq), K), padded(rows(wq), K), up(K, 1), type, e).view(result_shape(xq, wq.size(0)));
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_ffn, m) {
+  py::register_exception_translator([](std::exception_ptr p) {
+    try {
+      if (p) std::rethrow_exception(p);
+    } catch (const Refused& e) {
+      PyErr_SetString(error_type ? error_type : PyExc_RuntimeError, e.what());
+    }
+  });
+  m.def("bind", &bind);
+  m.def("set_timing", &set_timing);
+  m.def("rms_norm", &rms_norm);
+  m.def("rms_norm_quantized", &rms_norm_quantized);
+  m.def("quantize_rows", &quantize_rows);
+  m.def("linear_act", &linear_act);
+  m.def("linear_act_quantized", &linear_act_quantized);
+}
