@@ -120,7 +120,7 @@ class LinearArgs(ctypes.Structure):
     """mirror of hotk_linear_args (include/hotk.h)"""
     _fields_ = [('M', _L), ('N', _L), ('K', _L), ('x', _P), ('ld_x', _L), ('w', _P), ('ld_w', _L), ('bias', _P), ('res', _P),
                 ('ld_res', _L), ('y', _P), ('ld_y', _L), ('save', _P), ('x_scale', _P), ('w_scale', _P),
-                ('type', ctypes.c_int32), ('out_type', ctypes.c_int32), ('act', ctypes.c_int32), ('reserved', ctypes.c_int32)]
+                ('type', ctypes.c_int32), ('out_type', ctypes.c_int32), ('act', ctypes.c_int32), ('flags', ctypes.c_int32)]
 
 
 _SIGNATURES.update({
@@ -133,7 +133,9 @@ _SIGNATURES.update({
     'hotk_sum_partials': [_P, _L, _L, _P, _I, _P],
     'hotk_linear_workspace_bytes': [_L, _L, _L, _I, ctypes.POINTER(_S)],
     'hotk_linear_act': [ctypes.POINTER(LinearArgs), _P, _S, _P],
-    'hotk_linear_turn': [_P, _L, _P, _I, _P, _L, _P, _L, _P, _L, _L, _I, _P],
+    'hotk_linear_dz_partials': [_L, ctypes.POINTER(_L)],
+    'hotk_linear_dz': [_P, _L, _P, _I, _P, _L, _P, _L, _L, _I, _P],
+    'hotk_pad_rows': [_P, _L, _P, _L, _L, _L, _P],
 })
 EXPORTS = sorted(list(_SIGNATURES) + ['hotk_strerror', 'hotk_version'])
 
@@ -171,7 +173,7 @@ def torch_binding():
         from . import _ffn
     except ImportError as e:
         raise HotkError(f'hot_amd/_ffn is missing or does not load ({e}): build it with `python -m hot_amd.build`') from None
-    _ffn.bind({n: ctypes.cast(getattr(L, n), c_void_p).value for n in EXPORTS if n.startswith(('hotk_rmsnorm', 'hotk_quantize', 'hotk_sum_partials', 'hotk_linear_', 'hotk_strerror'))},
+    _ffn.bind({n: ctypes.cast(getattr(L, n), c_void_p).value for n in EXPORTS if n.startswith(('hotk_rmsnorm', 'hotk_quantize', 'hotk_sum_partials', 'hotk_linear_', 'hotk_pad_rows', 'hotk_strerror'))},
               HotkError)
     _ffn.set_timing(_timing_hook if _timing is not None else None)
     global _ffn_module

@@ -48,7 +48,9 @@ struct Entries {
   decltype(&hotk_sum_partials) sum_partials;
   decltype(&hotk_linear_workspace_bytes) linear_workspace_bytes;
   decltype(&hotk_linear_act) linear_act;
-  decltype(&hotk_linear_turn) linear_turn;
+  decltype(&hotk_linear_dz_partials) linear_dz_partials;
+  decltype(&hotk_linear_dz) linear_dz;
+  decltype(&hotk_pad_rows) pad_rows;
 } L{};
 
 template <class F>
@@ -67,7 +69,9 @@ void bind(const py::dict& d, py::object error) {
   bind_one(L.sum_partials, d, "hotk_sum_partials");
   bind_one(L.linear_workspace_bytes, d, "hotk_linear_workspace_bytes");
   bind_one(L.linear_act, d, "hotk_linear_act");
-  bind_one(L.linear_turn, d, "hotk_linear_turn");
+  bind_one(L.linear_dz_partials, d, "hotk_linear_dz_partials");
+  bind_one(L.linear_dz, d, "hotk_linear_dz");
+  bind_one(L.pad_rows, d, "hotk_pad_rows");
   error_type = error.release().ptr();      // kept for the process
 }
 
@@ -306,37 +310,21 @@ bool whole(const Rows& x, int64_t C) {     // rows as the product reads them: wh
   const int64_t e = x.t.element_size();
   return C * e % 16 == 0 && x.ld * e % 16 == 0 && (uintptr_t)x.p() % 16 == 0;
 }
-
-// v = in * slope -> any of out [R, ld_out], out_t [C, ld_t], column sums by 64 rows
-void turn(const Rows& in, int64_t C, const Tensor& save, int act, const Tensor& o, int64_t ld_o, const Tensor& o_t, int64_t ld_t,
-          const Tensor& part) {
-  launch("hotk_linear_turn", in.n * C * in.t.element_size() * (1 + o.defined() + o_t.defined()), [&] {
-    return L.linear_turn(in.p(), in.ld, out(save), act, out(o), ld_o, out(o_t), ld_t, (float*)out(part), in.n, C, type_of(in.t.scalar_type()),
-                         stream_of(in.t));
-  });
-}
-Rows turned(const Rows& in, int64_t C) {   // the transpose, rows of n padded with zeros to whole pieces
-  const int64_t ld = up(in.n, in.t.element_size());
-  const Tensor o = like(in.t, {C, ld}, in.t.scalar_type());
-  turn(in, C, {}, HOTK_ACT_NONE, {}, 0, o, ld, {});
-  return {o, ld, C};
-}
 Rows padded(const Rows& in, int64_t C) {   // itself where it is whole, else a copy with zeros behind each row
   if (in.n == 0 || whole(in, C)) return in;
-  const int64_t ld = up(C, in.t.element_size());
+  const int64_t e = in.t.element_size(), ld = up(C, e);
   const Tensor o = like(in.t, {in.n, ld}, in.t.scalar_type());
-  turn(in, C, {}, HOTK_ACT_NONE, o, ld, {}, 0, {});
+  launch("hotk_pad_rows", 2 * in.n * C * e, [&] { return L.pad_rows(in.p(), in.ld * e, o.data_ptr(), ld * e, in.n, C * e, stream_of(in.t)); });
   return {o, ld, in.n};
 }
 
 struct Extras {
   Tensor bias, save, x_scale, w_scale;
   Rows res;
-  int act = HOTK_ACT_NONE;
+  int act = HOTK_ACT_NONE, flags = 0;
 };
-// [x.n, w.n] = epilogue(x w^T); rows of K elements in whole pieces
-Tensor product(const Rows& x, const Rows& w, int64_t K, at::ScalarType type, const Extras& e) {
-  const int64_t M = x.n, N = w.n;
+// [M, N] = epilogue(x w^T), rows in whole pieces
+Tensor product(const Rows& x, const Rows& w, int64_t M, int64_t N, int64_t K, at::ScalarType type, const Extras& e) {
   const Tensor y = like(x.t, {M, N}, type);
   if (M == 0) return y;
   const int ty = type_of(x.t.scalar_type());
@@ -352,7 +340,7 @@ Tensor product(const Rows& x, const Rows& w, int64_t K, at::ScalarType type, con
   a.y = y.data_ptr(); a.ld_y = N;
   a.save = out(e.save);
   a.x_scale = (const float*)out(e.x_scale); a.w_scale = (const float*)out(e.w_scale);
-  a.type = ty; a.out_type = type_of(type); a.act = e.act;
+  a.type = ty; a.out_type = type_of(type); a.act = e.act; a.flags = e.flags;
   launch("hotk_linear_act", (M + N) * K * x.t.element_size() + M * N * y.element_size() * (1 + e.res.t.defined()),
          [&] { return L.linear_act(&a, out(ws), need, stream_of(x.t)); });
   return y;
@@ -390,7 +378,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& weight, const optional<Tens
   if (b) e.bias = b->contiguous();
   e.res = rows(r);
   if (grad && act) *save = e.save = like(x, {xs.n, N}, x.scalar_type() == at::kFloat ? at::kFloat : at::kShort);
-  return product(xs, ws, up(K, x.element_size()), x.scalar_type(), e).view(result_shape(x, N));
+  return product(xs, ws, xs.n, N, K, x.scalar_type(), e).view(result_shape(x, N));
 }
 
 struct LinearAct : torch::autograd::Function<LinearAct> {
@@ -415,28 +403,47 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     if (dy.defined() && (wants & 7)) {
       const c10::DeviceGuard guard(x.device());
       const auto type = x.scalar_type();
-      const int64_t size = x.element_size(), M = x.numel() / K;
+      const int64_t M = x.numel() / K;
       if (M == 0) {
         if (wants & 1) dx = at::zeros_like(x);
         if (wants & 2) dw = at::zeros_like(weight);
         if (wants & 4) db = at::zeros({N}, x.options());
       } else {
         const Rows gs = rows(dy);
-        const int64_t Np = up(N, size), Mp = up(M, size);
-        // one pass over dy: dz where it is not dy itself, its transpose for dw, its column sums
+        const int ty = type_of(type);
+        // one pass over dy: dz where it is not dy itself, and its column sums
+        Rows dz = gs;
         const bool itself = act == HOTK_ACT_NONE && whole(gs, N);
-        const Tensor dz = wants & 1 && !itself ? like(x, {M, Np}, type) : Tensor();
-        const Tensor dzt = wants & 2 ? like(x, {N, Mp}, type) : Tensor();
-        const Tensor part = wants & 4 ? like(x, {(M + 63) / 64, N}, at::kFloat) : Tensor();
-        if (dz.defined() || dzt.defined() || part.defined()) turn(gs, N, save, act, dz, Np, dzt, Mp, part);
+        if ((wants & 3) && !itself) {
+          const int64_t ld = up(N, x.element_size());
+          dz = {like(x, {M, ld}, type), ld, M};
+        }
+        Tensor part;
+        if (wants & 4) {
+          int64_t n = 0;
+          check(L.linear_dz_partials(M, &n), "hotk_linear_dz_partials");
+          part = like(x, {n, N}, at::kFloat);
+        }
+        const bool write = (wants & 3) && !itself;
+        if (write || part.defined())
+          launch("hotk_linear_dz", M * N * x.element_size() * (1 + write + (act != HOTK_ACT_NONE)), [&] {
+            return L.linear_dz(gs.p(), gs.ld, out(save), act, write ? dz.t.data_ptr() : nullptr, dz.ld, (float*)out(part), M, N, ty, stream_of(x));
+          });
         if (wants & 4) {
           db = like(x, {N}, type);
           launch("hotk_sum_partials", 4 * part.numel(), [&] {
-            return L.sum_partials(part.const_data_ptr<float>(), part.size(0), N, db.data_ptr(), type_of(type), stream_of(x));
+            return L.sum_partials(part.const_data_ptr<float>(), part.size(0), N, db.data_ptr(), ty, stream_of(x));
           });
         }
-        if (wants & 1) dx = product(itself ? gs : Rows{dz, Np, M}, turned(rows(weight), K), Np, type, {}).view(x.sizes());
-        if (wants & 2) dw = product({dzt, Mp, N}, turned(rows(x), K), Mp, type, {});
+        Extras e;
+        if (wants & 1) {
+          e.flags = HOTK_LINEAR_W_DOWN;
+          dx = product(dz, padded(rows(weight), K), M, K, N, type, e).view(x.sizes());
+        }
+        if (wants & 2) {
+          e.flags = HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN;
+          dw = product(dz, padded(rows(x), K), N, K, M, type, e);
+        }
       }
     }
     return {dx, dw, db, wants & 8 ? dy : Tensor(), Tensor()};
@@ -472,7 +479,7 @@ Tensor linear_act_quantized(const Tensor& xq, const Tensor& x_scale, const Tenso
   e.res = rows(r);
   e.x_scale = x_scale.contiguous();
   e.w_scale = w_scale.contiguous();
-  return product(padded(rows(xq), K), padded(rows(wq), K), up(K, 1), type, e).view(result_shape(xq, wq.size(0)));
+  return product(padded(rows(xq), K), padded(rows(wq), K), xq.numel() / K, wq.size(0), K, type, e).view(result_shape(xq, wq.size(0)));
 }
 
 }  // namespace

@@ -3,9 +3,8 @@
 //   z = x w^T + b (8-bit operands: z = sx_m sw_n (xq wq^T) + b)     y = f(z) + res        x [M, K], w [N, K], y [M, N]
 //   backward: dz = dy f'(z),  dx = dz w,  dw = dz^T x,  db = sum_m dz,  dres = dy
 //
-// One tile kernel for every type.  All operands have the contraction along their rows (dx and dw take transposed copies), a
-// tile row is 128 bytes of it = 64 16-bit, 32 fp32 or 128 8-bit elements, so loads, LDS image and fragment addresses are the
-// same bytes for all types and only the matrix instruction differs:
+// One tile kernel for every type and direction.  A tile step is 128 bytes of contraction (64 16-bit, 32 fp32 or 128 8-bit
+// elements), and only the matrix instruction differs between types:
 //   16-bit: 2 x v_mfma_f32_16x16x32,   fp32: 8 x v_mfma_f32_16x16x4_f32,   e4m3: 1 x v_mfma_f32_16x16x128_f8f6f4
 // (a contraction may take its terms in any order, so each type reads 16-byte pieces lane group by lane group).
 // The e4m3 instruction adds eight products at a time aligned to the largest of them and drops what is below 2^-13 of it
@@ -14,10 +13,17 @@
 // result would show it, so there the operands become bf16 (exactly: 4 significant bits) and 4 x v_mfma_f32_16x16x32_bf16 add
 // them in fp32.
 //
-// Tiles go global -> LDS by DMA, two stages, one barrier per step.  The DMA writes 64 consecutive 16-byte pieces, so the
-// swizzle that keeps fragment reads off each other's banks is applied to the SOURCE address: piece p of row r holds chunk
-// p ^ key(r).  The weight is the matrix instruction's row operand, its rows dealt to fragments so that a lane ends with 16
-// CONSECUTIVE output columns: bias, residual, y and the saved slope move in 16-byte accesses without a pass through LDS.
+// An operand has the contraction along its rows, or (dx reads w, dw reads dz and x that way) down its columns; the tile in LDS
+// keeps the operand's own order, and a transposed fragment is read by ds_read_b64_tr_b16 (16-bit) or as single floats (one
+// matrix instruction takes one float a lane), so no transposed copy is ever made.
+//
+// Tiles go global -> LDS by DMA, two stages.  The DMA writes 64 consecutive 16-byte pieces, so the swizzle that keeps fragment
+// reads off each other's banks is applied to the SOURCE address.  One barrier a step, placed before the step's last row of
+// matrix instructions: by then every fragment of the stage is in registers and the next stage has landed, so behind the
+// barrier the DMA of the step after next starts and the next step's first fragments are read while matrix instructions run.
+//
+// The weight is the matrix instruction's row operand; eight lane-group swaps then give a lane 16 consecutive output columns,
+// so bias, residual, y and the saved slope move in 16-byte accesses without a pass through LDS.
 //
 // For training, 16-bit types keep f'(z) as a 16-bit fixed-point number in steps of 2^-14 (|f'| < 1.13): its error of 2^-15
 // is far below the rounding of dz, where z rounded to the type would add as much as that rounding again, and the backward
@@ -46,49 +52,58 @@ __device__ __align__(16) const uint32_t la_zeros[4] = {0, 0, 0, 0};   // what li
 // ---- activations: f(z) and f'(z) ---------------------------------------------------------------------------------------
 // FAST (16-bit results): gelu by Abramowitz & Stegun 7.1.26 (|error of erf| <= 1.5e-7), whose exponential the slope shares;
 // tanh and the logistic function from one exponential.  fp32 results: the math library's functions.
-template <bool FAST>
-__device__ __forceinline__ float la_act(float z, int act, float& slope) {
-  switch (act) {
-    case HOTK_ACT_RELU: slope = z > 0.f ? 1.f : 0.f; return z < 0.f ? 0.f : z;       // (a NaN stays one)
-    case HOTK_ACT_LEAKYRELU: slope = z > 0.f ? 1.f : LA_LEAK; return z > 0.f ? z : LA_LEAK * z;
-    case HOTK_ACT_GELU: {
-      float cdf, pdf;
-      if (FAST) {
-        const float x = fabsf(z) * 0.70710678f;
-        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
-        const float e = __builtin_amdgcn_exp2f(-1.44269504f * x * x);
-        const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * e;
-        cdf = z < 0.f ? 0.5f * q : fmaf(-0.5f, q, 1.f);
-        pdf = 0.39894228f * e;
-      } else {
-        cdf = 0.5f * erfcf(-0.70710678f * z);
-        pdf = 0.39894228f * expf(-0.5f * z * z);
-      }
-      slope = fmaf(z, pdf, cdf);
-      return z * cdf;
+// ACT: HOTK_ACT_RELU stands for all three that are linear on either side of zero, with `neg` the slope below it.
+template <int ACT, bool FAST>
+__device__ __forceinline__ float la_act(float z, float neg, float& slope) {
+  if constexpr (ACT == HOTK_ACT_GELU) {
+    float cdf, pdf;
+    if (FAST) {
+      const float x = fabsf(z) * 0.70710678f;
+      const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+      const float e = __builtin_amdgcn_exp2f(-1.44269504f * x * x);
+      const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * e;
+      cdf = z < 0.f ? 0.5f * q : fmaf(-0.5f, q, 1.f);
+      pdf = 0.39894228f * e;
+    } else {
+      cdf = 0.5f * erfcf(-0.70710678f * z);
+      pdf = 0.39894228f * expf(-0.5f * z * z);
     }
-    case HOTK_ACT_TANH: {
-      float t;
-      if (FAST) {
-        const float s = z * z;
-        const float series = z * fmaf(s, fmaf(s, fmaf(s, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);   // to z^7: |z| < 1/4
-        const float e = __builtin_amdgcn_exp2f(2.88539008f * z);
-        const float quot = fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
-        t = fabsf(z) < 0.25f ? series : quot;
-      } else {
-        t = tanhf(z);
-      }
-      slope = fmaf(-t, t, 1.f);
-      return t;
+    slope = fmaf(z, pdf, cdf);
+    return z * cdf;
+  } else if constexpr (ACT == HOTK_ACT_TANH) {
+    float t;
+    if (FAST) {
+      const float s = z * z;
+      const float series = z * fmaf(s, fmaf(s, fmaf(s, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);   // to z^7: |z| < 1/4
+      const float e = __builtin_amdgcn_exp2f(2.88539008f * z);
+      const float quot = fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
+      t = fabsf(z) < 0.25f ? series : quot;
+    } else {
+      t = tanhf(z);
     }
-    case HOTK_ACT_SILU: {
-      const float e = FAST ? __builtin_amdgcn_exp2f(-1.44269504f * z) : expf(-z);
-      const float s = FAST ? __builtin_amdgcn_rcpf(1.f + e) : 1.f / (1.f + e);
-      slope = s * fmaf(z, 1.f - s, 1.f);
-      return z * s;
-    }
-    default: slope = 1.f; return z;
+    slope = fmaf(-t, t, 1.f);
+    return t;
+  } else if constexpr (ACT == HOTK_ACT_SILU) {
+    const float e = FAST ? __builtin_amdgcn_exp2f(-1.44269504f * z) : expf(-z);
+    const float s = FAST ? __builtin_amdgcn_rcpf(1.f + e) : 1.f / (1.f + e);
+    slope = s * fmaf(z, 1.f - s, 1.f);
+    return z * s;
+  } else {
+    slope = z > 0.f ? 1.f : neg;
+    return z > 0.f ? z : neg == 0.f ? (z <= 0.f ? 0.f : z) : neg * z;      // (relu: no infinity times zero, and a NaN stays one)
   }
+}
+__device__ __forceinline__ float la_neg(int act) { return act == HOTK_ACT_RELU ? 0.f : act == HOTK_ACT_LEAKYRELU ? LA_LEAK : 1.f; }
+template <bool FAST>
+__device__ __forceinline__ float la_act_grad(float z, int act) {
+  float d;
+  switch (act) {
+    case HOTK_ACT_GELU: la_act<HOTK_ACT_GELU, FAST>(z, 1.f, d); break;
+    case HOTK_ACT_TANH: la_act<HOTK_ACT_TANH, FAST>(z, 1.f, d); break;
+    case HOTK_ACT_SILU: la_act<HOTK_ACT_SILU, FAST>(z, 1.f, d); break;
+    default: la_act<HOTK_ACT_RELU, FAST>(z, la_neg(act), d);
+  }
+  return d;
 }
 __device__ __forceinline__ int16_t la_slope_code(float d) {
   const int c = (int)rintf(d * (1.f / LA_SLOPE_STEP));
@@ -111,11 +126,45 @@ struct LaEpi {
   int act;
 };
 
-// W consecutive columns (a multiple of 8) of one row, from n0: z is the bare product
+// a piece of W values of a row as 16-byte accesses
+template <int ACT, int W, class OT>
+__device__ __forceinline__ void la_activate(const LaEpi<OT>& e, int64_t m, int64_t n0, int64_t N, int left, float (&z)[W]) {
+  constexpr bool FAST = !std::is_same<OT, float>::value;
+  const float neg = la_neg(e.act);
+  float d[W];
+  if (!FAST && e.save && e.act != HOTK_ACT_NONE) {
+    float* row = (float*)e.save + m * N + n0;
+#pragma unroll
+    for (int i = 0; i < W; i += 4)
+      if (i < left) ffn_store(row, i, left, f32x4{z[i], z[i + 1], z[i + 2], z[i + 3]});
+  }
+#pragma unroll
+  for (int i = 0; i < W; ++i) z[i] = la_act<ACT, FAST>(z[i], neg, d[i]);
+  if (FAST && e.save && e.act != HOTK_ACT_NONE) {
+    typedef int16_t s16x8 __attribute__((ext_vector_type(8)));
+    typedef int16_t s16x8u __attribute__((ext_vector_type(8), aligned(2)));
+    int16_t* row = (int16_t*)e.save + m * N + n0;
+#pragma unroll
+    for (int i = 0; i < W; i += 8) {
+      s16x8 c;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) c[k] = la_slope_code(d[i + k]);
+      if (i + 8 <= left) {
+        *reinterpret_cast<s16x8u*>(row + i) = c;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (i + k < left) row[i + k] = c[k];
+      }
+    }
+  }
+}
+
+// W consecutive columns (a multiple of 8) of one row, from n0: z is the bare product.  The activation is chosen once per piece:
+// W independent chains run side by side
 template <int W, class OT>
 __device__ __forceinline__ void la_finish(const LaEpi<OT>& e, int64_t m, int64_t n0, int64_t N, float (&z)[W]) {
   using E = Elem<OT>;
-  constexpr bool FAST = !std::is_same<OT, float>::value;
   const int left = (int)(N - n0 < W ? N - n0 : W);               // columns of this piece that exist
   if (left <= 0) return;
   if (e.xs) {
@@ -135,51 +184,12 @@ __device__ __forceinline__ void la_finish(const LaEpi<OT>& e, int64_t m, int64_t
       for (int k = 0; k < E::VEC; ++k) z[i + k] += b[k];
     }
   }
-  if (e.act != HOTK_ACT_NONE) {
-    if (e.save) {
-      if (FAST) {
-        int16_t* row = (int16_t*)e.save + m * N + n0;
-        typedef int16_t s16x8 __attribute__((ext_vector_type(8)));
-        typedef int16_t s16x8u __attribute__((ext_vector_type(8), aligned(2)));
-#pragma unroll
-        for (int i = 0; i < W; i += 8) {
-          s16x8 c;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            float d;
-            z[i + k] = la_act<FAST>(z[i + k], e.act, d);
-            c[k] = la_slope_code(d);
-          }
-          if (i + 8 <= left) {
-            *reinterpret_cast<s16x8u*>(row + i) = c;
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (i + k < left) row[i + k] = c[k];
-          }
-        }
-      } else {
-        float* row = (float*)e.save + m * N + n0;
-#pragma unroll
-        for (int i = 0; i < W; i += 4) {
-          f32x4 c;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) c[k] = z[i + k];
-          if (i < left) ffn_store(row, i, left, c);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float d;
-            z[i + k] = la_act<FAST>(z[i + k], e.act, d);
-          }
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        float d;
-        z[i] = la_act<FAST>(z[i], e.act, d);
-      }
-    }
+  switch (e.act) {
+    case HOTK_ACT_NONE: break;
+    case HOTK_ACT_GELU: la_activate<HOTK_ACT_GELU>(e, m, n0, N, left, z); break;
+    case HOTK_ACT_TANH: la_activate<HOTK_ACT_TANH>(e, m, n0, N, left, z); break;
+    case HOTK_ACT_SILU: la_activate<HOTK_ACT_SILU>(e, m, n0, N, left, z); break;
+    default: la_activate<HOTK_ACT_RELU>(e, m, n0, N, left, z);
   }
 #pragma unroll
   for (int i = 0; i < W; i += E::VEC) {
@@ -194,10 +204,9 @@ __device__ __forceinline__ void la_finish(const LaEpi<OT>& e, int64_t m, int64_t
 // ---- the tile kernel ---------------------------------------------------------------------------------------------------
 template <class OT>
 struct LaTile {
-  const char *a, *b;             // x [M, K], w [N, K]
+  const char *a, *b;             // x [M, K] or [K, M], w [N, K] or [K, N]
   int64_t lda, ldb;              // bytes per row
-  int64_t M, N;
-  int chunks;                    // 16-byte pieces of a row
+  int64_t M, N, K;
   int ktiles, kper;              // 128-byte steps, and how many of them a split takes
   int tiles_m, tiles_n;
   float* part;                   // [splits][M][N] bare products, where there is more than one split
@@ -221,13 +230,56 @@ __device__ __forceinline__ void la_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)
 // workgroup barrier behind this wave's LDS reads, silent about the loads in flight
 __device__ __forceinline__ void la_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 
-// chunk p ^ key of a row sits at piece p.  x fragments read 16 consecutive rows, w fragments rows {0..3} + 16 {0..3}
-__device__ __forceinline__ int la_key_x(int row) { return row & 7; }
-__device__ __forceinline__ int la_key_w(int row) { return (row & 3) | ((row >> 2) & 4); }
+// An operand tile in LDS: BLK columns by one step.  Along rows (T false): BLK rows of 8 pieces, piece p of row r holds chunk
+// p ^ (r & 7).  Down columns (T true): a step's rows of BLK elements; blocks of 16 elements are exchanged by a key of the row,
+// such that the rows which a fragment read touches at once lie in different banks.
+template <class IT> struct LaBytes { static constexpr int E = 2; };
+template <> struct LaBytes<float> { static constexpr int E = 4; };
+template <> struct LaBytes<e4m3> { static constexpr int E = 1; };
+template <> struct LaBytes<e4m3_wide> { static constexpr int E = 1; };
 
-__device__ __forceinline__ u32x4 la_frag(const unsigned char* tile, int row, int chunk, int key) {
-  return *reinterpret_cast<const u32x4*>(tile + row * 128 + ((chunk ^ key) << 4));
-}
+template <class IT, bool T, int BLK>
+struct LaSide {
+  static constexpr int E = LaBytes<IT>::E, STEP = 128 / E;       // elements of contraction a step
+  static constexpr int PPR = T ? BLK * E / 16 : 8;               // pieces per row of the tile
+  static constexpr int PPB = E;                                  // pieces per block of 16 elements (T)
+  static __device__ __forceinline__ int key(int k) {
+    return (E == 2 ? (k & 3) | ((k >> 1) & 4) : (k >> 2) & 3) & (BLK / 16 - 1);
+  }
+  // piece number `piece` of the tile: its row of the operand's tile, and which chunk of that row it holds
+  static __device__ __forceinline__ void source(int piece, int& row, int& chunk) {
+    row = piece / PPR;
+    const int pos = piece % PPR;
+    if (T) chunk = (((pos / PPB) ^ key(row)) * PPB) | (pos % PPB);
+    else chunk = pos ^ (row & 7);
+  }
+  // 16 bytes of contraction of column col0 + lr, piece 4 h + lg
+  static __device__ __forceinline__ u32x4 frag(const unsigned char* tile, int col0, int h, int lr, int lg) {
+    u32x4 v;
+    if constexpr (!T) {
+      const int row = col0 + lr;
+      v = *reinterpret_cast<const u32x4*>(tile + row * 128 + (((4 * h + lg) ^ (row & 7)) << 4));
+    } else if constexpr (E == 2) {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {      // lane 4 r + c of a group brings columns 4 c .. of row r and leaves with a column of four rows
+        const int k = 32 * h + 8 * lg + 4 * q + (lr >> 2), col = col0 + 4 * (lr & 3);
+        const unsigned char* at = tile + k * (BLK * 2) + (((col >> 4) ^ key(k)) << 5) + (col & 15) * 2;
+        const u32x2 t = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
+        v[2 * q] = t[0];
+        v[2 * q + 1] = t[1];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = 16 * h + 4 * lg + i, col = col0 + lr;
+        v[i] = *reinterpret_cast<const uint32_t*>(tile + k * (BLK * 4) + (((col >> 4) ^ key(k)) << 6) + (col & 15) * 4);
+      }
+    }
+    return v;
+  }
+};
 
 // what a lane holds of a fragment: two 16-byte pieces, or their elements in bf16
 template <class IT>
@@ -287,11 +339,53 @@ __device__ __forceinline__ void la_tile_of(int pid, int tiles_m, int tiles_n, in
   in = in_group / rows;
 }
 
-template <class IT, class OT, int BM, int BN, int WM, int WN>
+// one operand's part of the DMA: its pieces for this lane and where they come from
+template <class IT, bool T, int BLK, int NW>
+struct LaFeed {
+  using S = LaSide<IT, T, BLK>;
+  static constexpr int LOADS = BLK * 8 / 64 / NW;
+  static_assert(BLK * 8 % (64 * NW) == 0, "whole DMA instructions per wave");
+  const char* base;
+  int64_t ld;
+  uint32_t off[LOADS];
+  int wave, lane;
+  // columns past the operand's end repeat its last row (T: piece); their products are not stored
+  __device__ __forceinline__ LaFeed(const char* p, int64_t ld_, int64_t col0, int64_t cols, int wave_, int lane_)
+      : base(T ? p + col0 * S::E : p + col0 * ld_), ld(ld_), wave(wave_), lane(lane_) {
+    const int64_t left = cols - col0;
+    const int last = T ? (int)((left < BLK ? left : BLK) * S::E + 15) / 16 - 1 : (int)(left < BLK ? left : BLK) - 1;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      int row, chunk;
+      S::source((wave + NW * i) * 64 + lane, row, chunk);
+      if (T) chunk = chunk < last ? chunk : last;
+      else row = row < last ? row : last;
+      off[i] = (uint32_t)(row * ld) + chunk * 16;
+    }
+  }
+  __device__ __forceinline__ void issue(int kt, int64_t K, uint32_t dst) const {
+    const char* at = base + (T ? (int64_t)kt * S::STEP * ld : (int64_t)kt * 128);
+    if ((int64_t)(kt + 1) * S::STEP <= K) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) la_dma(at, off[i], dst + (wave + NW * i) * 1024);
+    } else {                             // the last step: zeros where the contraction has ended
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        int row, chunk;
+        S::source((wave + NW * i) * 64 + lane, row, chunk);
+        const int64_t k = (int64_t)kt * S::STEP + (T ? row : chunk * (16 / S::E));
+        la_dma_at(k < K ? at + off[i] : (const char*)la_zeros, dst + (wave + NW * i) * 1024);
+      }
+    }
+  }
+};
+
+template <class IT, class OT, bool TA, bool TB, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_linact_tile(const LaTile<OT> g) {
   constexpr int NW = WM * WN, TM = BM / WM, MF = TM / 16, NF = 4, STAGE = (BM + BN) * 128;
-  constexpr int PIECES = (BM + BN) / 8, LOADS = PIECES / NW;     // a wave's DMA instructions per step: 8 rows each
-  static_assert(BN / WN == 64 && PIECES % NW == 0 && BM % (16 * WM) == 0, "a wave owns 64 columns");
+  static_assert(BN / WN == 64 && BM % (16 * WM) == 0, "a wave owns 64 columns");
+  using SA = LaSide<IT, TA, BM>;
+  using SB = LaSide<IT, TB, BN>;
   extern __shared__ __align__(16) unsigned char lds[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -300,37 +394,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linact_tile(const LaTile<OT> g
   la_tile_of(blockIdx.x, g.tiles_m, g.tiles_n, im, in);
   const int64_t m0 = (int64_t)im * BM, n0 = (int64_t)in * BN;
   const int k0 = blockIdx.y * g.kper, k1 = min(g.ktiles, k0 + g.kper);
-  const char* abase = g.a + m0 * g.lda;
-  const char* bbase = g.b + n0 * g.ldb;
-
-  // this lane's source offsets: piece group i of the wave = rows 8 (wave + NW i) .. + 8 of [x tile | w tile]; rows past the
-  // end repeat the last one (their products are not stored)
-  uint32_t off[LOADS];
-#pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    const int p = wave + NW * i;
-    const bool is_x = p < BM / 8;
-    const int row = (is_x ? p : p - BM / 8) * 8 + (lane >> 3);
-    const int chunk = (lane & 7) ^ (is_x ? la_key_x(row) : la_key_w(row));
-    const int64_t last = (is_x ? g.M - m0 : g.N - n0) - 1;
-    off[i] = (uint32_t)((row < last ? row : last) * (is_x ? g.lda : g.ldb)) + chunk * 16;
-  }
+  const LaFeed<IT, TA, BM, NW> fa(g.a, g.lda, m0, g.M, wave, lane);
+  const LaFeed<IT, TB, BN, NW> fb(g.b, g.ldb, n0, g.N, wave, lane);
   auto issue = [&](int kt, int stage) {
-    const bool whole = kt * 8 + 8 <= g.chunks;
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int p = wave + NW * i;
-      const bool is_x = p < BM / 8;
-      const char* base = (is_x ? abase : bbase) + (int64_t)kt * 128;
-      const uint32_t dst = lds0 + stage * STAGE + p * 1024;
-      if (whole) {
-        la_dma(base, off[i], dst);
-      } else {
-        const int row = (is_x ? p : p - BM / 8) * 8 + (lane >> 3);
-        const int chunk = (lane & 7) ^ (is_x ? la_key_x(row) : la_key_w(row));
-        la_dma_at(kt * 8 + chunk < g.chunks ? base + off[i] : (const char*)la_zeros, dst);
-      }
-    }
+    fa.issue(kt, g.K, lds0 + stage * STAGE);
+    fb.issue(kt, g.K, lds0 + stage * STAGE + BM * 128);
   };
 
   f32x4 acc[MF][NF];
@@ -338,30 +406,49 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linact_tile(const LaTile<OT> g
   for (int i = 0; i < MF; ++i)
 #pragma unroll
     for (int j = 0; j < NF; ++j) acc[i][j] = 0.f;
-
-  if (k0 < k1) issue(k0, 0);
-  for (int kt = k0; kt < k1; ++kt) {
-    const int stage = (kt - k0) & 1;
-    la_wait_vm<0>();       // this wave's part of the step has landed,
-    la_barrier();          // everyone's has, and everyone has read the other stage
-    if (kt + 1 < k1) issue(kt + 1, stage ^ 1);
-    const unsigned char* xt = lds + stage * STAGE;
-    const unsigned char* wt = xt + BM * 128;
-    LaFrag<IT> wf[NF];
+  LaFrag<IT> wf[2][NF], xf[2];
+  auto read_w = [&](int stage, LaFrag<IT>(&f)[NF]) {
 #pragma unroll
-    for (int j = 0; j < NF; ++j) {
-      const int row = wn * 64 + 16 * (lr >> 2) + 4 * j + (lr & 3);
+    for (int j = 0; j < NF; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) wf[j].set(h, la_frag(wt, row, 4 * h + lg, la_key_w(row)));
-    }
+      for (int h = 0; h < 2; ++h) f[j].set(h, SB::frag(lds + stage * STAGE + BM * 128, wn * 64 + 16 * j, h, lr, lg));
+  };
+  auto read_x = [&](int stage, int i, LaFrag<IT>& f) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) f.set(h, SA::frag(lds + stage * STAGE, wm * TM + 16 * i, h, lr, lg));
+  };
+  // step kt from stage S: fragments 0 are in registers.  Before the last row of matrix instructions the stage has been read
+  // whole, and step kt + 1 has landed in the other
+  auto step = [&](int kt, auto stage_tag) {
+    constexpr int S = decltype(stage_tag)::value;
 #pragma unroll
     for (int i = 0; i < MF; ++i) {
-      const int row = wm * TM + 16 * i + lr;
-      LaFrag<IT> xf;
+      if (i + 1 < MF) {
+        read_x(S, i + 1, xf[(i + 1) & 1]);
+      } else if (kt + 1 < k1) {
+        la_wait_vm<0>();
+        la_barrier();
+        if (kt + 2 < k1) issue(kt + 2, S);
+        read_w(S ^ 1, wf[S ^ 1]);
+        read_x(S ^ 1, 0, xf[MF > 1 ? 0 : 1]);
+      }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) xf.set(h, la_frag(xt, row, 4 * h + lg, la_key_x(row)));
-#pragma unroll
-      for (int j = 0; j < NF; ++j) la_mma<IT>(acc[i][j], wf[j], xf);
+      for (int j = 0; j < NF; ++j) la_mma<IT>(acc[i][j], wf[S][j], xf[i & 1]);
+    }
+    if (MF == 1) xf[0] = xf[1];
+  };
+  static_assert(MF == 1 || MF % 2 == 0, "the first fragment of a step is in xf[0]");
+
+  if (k0 < k1) {
+    issue(k0, 0);
+    la_wait_vm<0>();
+    la_barrier();
+    if (k0 + 1 < k1) issue(k0 + 1, 1);
+    read_w(0, wf[0]);
+    read_x(0, 0, xf[0]);
+    for (int kt = k0; kt < k1; kt += 2) {
+      step(kt, std::integral_constant<int, 0>{});
+      if (kt + 1 < k1) step(kt + 1, std::integral_constant<int, 1>{});
     }
   }
 
@@ -369,20 +456,26 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linact_tile(const LaTile<OT> g
 #pragma unroll
   for (int i = 0; i < MF; ++i) {
     const int64_t m = m0 + wm * TM + 16 * i + lr;
+    // lane group q holds columns 4 q .. of each of the four fragments: swapped so that group q holds the 16 columns of fragment q
     float z[16];
 #pragma unroll
-    for (int j = 0; j < NF; ++j)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) z[4 * j + k] = acc[i][j][k];
+    for (int k = 0; k < 4; ++k) {
+      const auto u02 = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][0][k]), __float_as_uint(acc[i][2][k]), false, false);
+      const auto u13 = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][1][k]), __float_as_uint(acc[i][3][k]), false, false);
+      const auto lo = __builtin_amdgcn_permlane16_swap(u02[0], u13[0], false, false);
+      const auto hi = __builtin_amdgcn_permlane16_swap(u02[1], u13[1], false, false);
+      z[k] = __uint_as_float(lo[0]);
+      z[4 + k] = __uint_as_float(lo[1]);
+      z[8 + k] = __uint_as_float(hi[0]);
+      z[12 + k] = __uint_as_float(hi[1]);
+    }
     if (m >= g.M) continue;
     if (g.part) {
       float* row = g.part + ((int64_t)blockIdx.y * g.M + m) * g.N + n;
       const int left = (int)(g.N - n < 16 ? g.N - n : 16);
 #pragma unroll
-      for (int j = 0; j < 16; j += 4) {
-        const f32x4 v = {z[j], z[j + 1], z[j + 2], z[j + 3]};
-        if (j < left) ffn_store(row, j, left, v);
-      }
+      for (int j = 0; j < 16; j += 4)
+        if (j < left) ffn_store(row, j, left, f32x4{z[j], z[j + 1], z[j + 2], z[j + 3]});
     } else {
       la_finish<16>(g.e, m, n, g.N, z);
     }
@@ -411,46 +504,80 @@ __global__ __launch_bounds__(256) void k_linact_join(const float* __restrict__ p
   }
 }
 
-// ---- backward: dz and its transpose, transposed and padded copies --------------------------------------------------------
-// 64 x 64 tiles through LDS.  in [R, C] -> (MODE >= 1: times the saved slope) -> out [R, ld_out] and / or out_t [C, ld_t], both
-// with zeros up to their row length, and column sums of each tile, partial [tile row][C]
-template <class T, bool DZ>
-__global__ __launch_bounds__(256) void k_linact_turn(const T* __restrict__ in, int64_t ld_in, const void* __restrict__ save, int act,
-                                                     T* __restrict__ out, int64_t ld_out, T* __restrict__ out_t, int64_t ld_t,
-                                                     float* __restrict__ partial, int64_t R, int64_t C, unsigned across) {
-  __shared__ T tile[64][65];
-  __shared__ float sums[4][64];
-  const int64_t down = blockIdx.x / across, r0 = down * 64, c0 = (int64_t)(blockIdx.x % across) * 64;
-  const int cx = threadIdx.x & 63, ry = threadIdx.x >> 6;
-  float s = 0.f;
-  for (int i = ry; i < 64; i += 4) {
-    const int64_t r = r0 + i, c = c0 + cx;
-    float v = 0.f;
-    if (r < R && c < C) {
-      v = (float)in[r * ld_in + c];
-      if (DZ && act != HOTK_ACT_NONE) {
-        if (std::is_same<T, float>::value) {
-          float d;
-          la_act<false>(((const float*)save)[r * C + c], act, d);
-          v *= d;
-        } else {
-          v *= la_slope(((const int16_t*)save)[r * C + c], act);
+// ---- backward: dz and its column sums; rows padded to whole pieces ---------------------------------------------------------
+// v = in * slope over a block of `rows` rows: out [R, ld_out] with zeros from C on, partial [block][C] the block's column sums.
+// A thread owns one 16-byte piece of columns and every (256 / cg)th row of the block; cg (a power of two) pieces go side by side
+template <class T>
+__global__ __launch_bounds__(256) void k_linact_dz(const T* __restrict__ in, int64_t ld_in, const void* __restrict__ save, int act,
+                                                   T* __restrict__ out, int64_t ld_out, float* __restrict__ partial, int64_t R,
+                                                   int64_t C, int rows, int cg_log, unsigned across) {
+  using E = Elem<T>;
+  using FV = typename E::fvec;
+  __shared__ FV sums[256];
+  const int cg = 1 << cg_log, piece = threadIdx.x & (cg - 1), rl = threadIdx.x >> cg_log, rstep = 256 >> cg_log;
+  const int64_t block = blockIdx.x / across, c = ((int64_t)(blockIdx.x % across) * cg + piece) * E::VEC;
+  const int64_t r1 = (block + 1) * rows < R ? (block + 1) * rows : R;
+  const int left = (int)(C - c < E::VEC ? (C > c ? C - c : 0) : E::VEC), room = (int)(ld_out - c < E::VEC ? (ld_out > c ? ld_out - c : 0) : E::VEC);
+  FV s = 0.f;
+  if (left > 0 || (out && room > 0)) {
+#pragma unroll 2
+    for (int64_t r = block * rows + rl; r < r1; r += rstep) {
+      FV v = 0.f;
+      if (left > 0) {
+        v = ffn_load(in + r * ld_in + c, 0, left);
+        if (act != HOTK_ACT_NONE) {
+          if constexpr (std::is_same<T, float>::value) {
+            const f32x4 z = ffn_load((const float*)save + r * C + c, 0, left);
+#pragma unroll
+            for (int k = 0; k < E::VEC; ++k) v[k] *= la_act_grad<false>(z[k], act);
+          } else {
+            typedef int16_t s16x8u __attribute__((ext_vector_type(8), aligned(2)));
+            const int16_t* codes = (const int16_t*)save + r * C + c;
+            if (left == E::VEC) {
+              const s16x8u d = *reinterpret_cast<const s16x8u*>(codes);
+#pragma unroll
+              for (int k = 0; k < E::VEC; ++k) v[k] *= la_slope(d[k], act);
+            } else {
+#pragma unroll
+              for (int k = 0; k < E::VEC; ++k)
+                if (k < left) v[k] *= la_slope(codes[k], act);
+            }
+          }
         }
+        s += v;
       }
+      if (out && room > 0) ffn_store(out + r * ld_out + c, 0, room, v);
     }
-    const T t = (T)v;
-    s += v;
-    if (out && r < R && c < ld_out) out[r * ld_out + c] = t;
-    tile[i][cx] = t;
   }
-  if (partial) sums[ry][cx] = s;
-  __syncthreads();
-  if (partial && ry == 0 && r0 < R && c0 + cx < C) partial[down * C + c0 + cx] = (sums[0][cx] + sums[1][cx]) + (sums[2][cx] + sums[3][cx]);
-  if (out_t)
-    for (int i = ry; i < 64; i += 4) {
-      const int64_t c = c0 + i, r = r0 + cx;
-      if (c < C && r < ld_t) out_t[c * ld_t + r] = tile[cx][i];
+  if (partial) {
+    sums[threadIdx.x] = s;
+    __syncthreads();
+    if (rl == 0) {
+      for (int i = 1; i < rstep; ++i) s += sums[(i << cg_log) + piece];
+#pragma unroll
+      for (int k = 0; k < E::VEC; ++k)
+        if (k < left) partial[block * C + c + k] = s[k];
     }
+  }
+}
+
+// a copy of rows of `bytes` bytes with zeros behind them up to ld_out, 16 bytes a thread
+__global__ __launch_bounds__(256) void k_pad_rows(const uint8_t* __restrict__ in, int64_t ld_in, uint8_t* __restrict__ out, int64_t ld_out,
+                                                  int64_t R, int64_t bytes) {
+  typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(1)));
+  const int64_t per_row = ld_out / 16, total = R * per_row;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+    const int64_t r = t / per_row, c = t % per_row * 16;
+    const uint8_t* src = in + r * ld_in + c;
+    u32x4 v = 0;
+    if (c + 16 <= bytes) {
+      v = *reinterpret_cast<const u32x4u*>(src);
+    } else {
+      for (int i = 0; i < 16; ++i)
+        if (c + i < bytes) v[i / 4] |= (uint32_t)src[i] << (8 * (i % 4));
+    }
+    *reinterpret_cast<u32x4*>(out + r * ld_out + c) = v;
+  }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
@@ -461,7 +588,8 @@ struct LaShape { int bm, bn, splits; };
 LaShape la_shape(int64_t M, int64_t N, int64_t ktiles) {
   LaShape s{256, 256, 1};
   if (la_div(M, 256) * la_div(N, 256) < 192) s = {128, 128, 1};
-  if (M <= 64) s = {32, 128, 1};
+  if (la_div(M, 128) * la_div(N, 128) < 128) s = {64, 64, 1};
+  if (M <= 32) s = {32, 128, 1};
   const int64_t tiles = la_div(M, s.bm) * la_div(N, s.bn);
   // fewer tiles than compute units: the contraction is split until there is one workgroup each, four steps or more a split
   if (tiles < 192) {
@@ -473,10 +601,10 @@ LaShape la_shape(int64_t M, int64_t N, int64_t ktiles) {
   return s;
 }
 
-template <class IT, class OT, int BM, int BN, int WM, int WN>
+template <class IT, class OT, bool TA, bool TB, int BM, int BN, int WM, int WN>
 int la_run(LaTile<OT>& g, int splits, hipStream_t st) {
   constexpr int LDS = 2 * (BM + BN) * 128;
-  auto kernel = k_linact_tile<IT, OT, BM, BN, WM, WN>;
+  auto kernel = k_linact_tile<IT, OT, TA, TB, BM, BN, WM, WN>;
   if (LDS > 64 * 1024) {                 // more LDS than a kernel gets without asking: asked for once per device
     static std::atomic<uint64_t> asked{0};
     int dev = 0;
@@ -493,23 +621,24 @@ int la_run(LaTile<OT>& g, int splits, hipStream_t st) {
   return hotk_launch_status();
 }
 
-template <class IT, class OT>
+template <class IT, class OT, bool TA, bool TB>
 int la_product(const hotk_linear_args& a, void* ws, size_t nws, hipStream_t st) {
   const int e = ffn_bytes(a.type);
-  const int64_t chunks = a.K * e / 16, ktiles = la_div(chunks, 8);
+  const int64_t ktiles = la_div(a.K * e, 128);
   const LaShape s = la_shape(a.M, a.N, ktiles);
   const size_t need = s.splits > 1 ? (size_t)s.splits * a.M * a.N * 4 : 0;
   if (nws < need || (need && !ws)) return HOTK_EWORKSPACE;
   LaTile<OT> g{};
   g.a = (const char*)a.x; g.b = (const char*)a.w;
   g.lda = a.ld_x * e; g.ldb = a.ld_w * e;
-  g.M = a.M; g.N = a.N;
-  g.chunks = (int)chunks; g.ktiles = (int)ktiles; g.kper = (int)la_div(ktiles, s.splits);
+  g.M = a.M; g.N = a.N; g.K = a.K;
+  g.ktiles = (int)ktiles; g.kper = (int)la_div(ktiles, s.splits);
   g.part = need ? (float*)ws : nullptr;
   g.e = {(const OT*)a.bias, (const OT*)a.res, a.ld_res, (OT*)a.y, a.ld_y, a.save, a.x_scale, a.w_scale, a.act};
-  int rc = s.bm == 256 ? la_run<IT, OT, 256, 256, 2, 4>(g, s.splits, st)
-         : s.bm == 128 ? la_run<IT, OT, 128, 128, 2, 2>(g, s.splits, st)
-                       : la_run<IT, OT, 32, 128, 2, 2>(g, s.splits, st);
+  int rc = s.bm == 256 ? la_run<IT, OT, TA, TB, 256, 256, 2, 4>(g, s.splits, st)
+         : s.bm == 128 ? la_run<IT, OT, TA, TB, 128, 128, 2, 2>(g, s.splits, st)
+         : s.bm == 64 ? la_run<IT, OT, TA, TB, 64, 64, 2, 1>(g, s.splits, st)
+                      : la_run<IT, OT, TA, TB, 32, 128, 2, 2>(g, s.splits, st);
   if (rc == HOTK_OK && need) {
     const int64_t work = a.M * la_div(a.N, 8);
     hipLaunchKernelGGL(k_linact_join<OT>, dim3(hotk_grid(work, 256)), dim3(256), 0, st, (const float*)ws, s.splits, a.M, a.N, g.e);
@@ -522,23 +651,31 @@ int la_check(const hotk_linear_args& a) {
   HOTK_CHECK_ARG(a.M >= 0 && a.N > 0 && a.K > 0);
   if (!(ffn_type_ok(a.type) || a.type == HOTK_E4M3) || !ffn_type_ok(a.out_type)) return HOTK_EUNSUPPORTED;
   if (a.type != HOTK_E4M3 && a.out_type != a.type) return HOTK_EUNSUPPORTED;
+  HOTK_CHECK_ARG((a.flags & ~(HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN)) == 0);
+  if (a.flags == HOTK_LINEAR_X_DOWN || (a.flags && a.type == HOTK_E4M3)) return HOTK_EUNSUPPORTED;
   HOTK_CHECK_ARG(a.act >= HOTK_ACT_NONE && a.act <= HOTK_ACT_SILU);
   HOTK_CHECK_ARG((a.type == HOTK_E4M3) == (a.x_scale != nullptr) && (a.x_scale != nullptr) == (a.w_scale != nullptr));
   HOTK_CHECK_ARG(a.type != HOTK_E4M3 || !a.save);
-  const int e = ffn_bytes(a.type);
-  HOTK_CHECK_ARG(a.ld_x >= a.K && a.ld_w >= a.K && a.ld_y >= a.N && (!a.res || a.ld_res >= a.N));
-  // contraction rows in whole, aligned 16-byte pieces (the caller pads others: hotk_linear_turn)
-  if ((a.K * e) % 16 || (a.ld_x * e) % 16 || (a.ld_w * e) % 16) return HOTK_EUNSUPPORTED;
+  const int e = ffn_bytes(a.type), m = 16 / e;
+  // operands in rows of whole, aligned 16-byte pieces (the caller pads others: hotk_pad_rows)
+  const int64_t row_x = a.flags & HOTK_LINEAR_X_DOWN ? a.M : a.K, row_w = a.flags & HOTK_LINEAR_W_DOWN ? a.N : a.K;
+  HOTK_CHECK_ARG(a.ld_x >= row_x && a.ld_w >= row_w && a.ld_y >= a.N && (!a.res || a.ld_res >= a.N));
+  if (a.ld_x < la_div(row_x, m) * m || a.ld_w < la_div(row_w, m) * m || (a.ld_x * e) % 16 || (a.ld_w * e) % 16) return HOTK_EUNSUPPORTED;
   if (a.M > 0) {
     HOTK_CHECK_ARG(a.x && a.w && a.y);
     if (!hotk_aligned16(a.x) || !hotk_aligned16(a.w)) return HOTK_EUNSUPPORTED;
     HOTK_CHECK_ARG(ffn_elem_aligned(a.y, a.out_type) && ffn_elem_aligned(a.bias, a.out_type) && ffn_elem_aligned(a.res, a.out_type));
-    HOTK_CHECK_ARG(((uintptr_t)a.save) % 4 == 0 || a.out_type != HOTK_F32);
+    HOTK_CHECK_ARG(((uintptr_t)a.save) % (a.out_type == HOTK_F32 ? 4 : 2) == 0);
+    HOTK_CHECK_ARG(((uintptr_t)a.x_scale) % 4 == 0 && ((uintptr_t)a.w_scale) % 4 == 0);
   }
-  // 32-bit offsets inside a tile, 32-bit tile counts
-  if (a.ld_x * e > (1 << 23) || a.ld_w * e > (1 << 23) || la_div(a.M, 32) * la_div(a.N, 128) > (1ll << 30)) return HOTK_ETOOLARGE;
+  // 32-bit offsets inside a tile, 32-bit tile and step counts
+  if (a.ld_x * e > (1 << 23) || a.ld_w * e > (1 << 23) || la_div(a.M, 32) * la_div(a.N, 64) > (1ll << 30) || la_div(a.K * e, 128) > (1ll << 30))
+    return HOTK_ETOOLARGE;
   return HOTK_OK;
 }
+
+// rows of a block of hotk_linear_dz: 64, and more where that would be over 1024 blocks of column sums
+int64_t la_dz_rows(int64_t R) { return la_div(la_div(R, 1024), 64) * 64; }
 
 }  // namespace
 
@@ -559,33 +696,48 @@ extern "C" int hotk_linear_act(const hotk_linear_args* args, void* workspace, si
   ffn_dispatch(args->out_type, [&](auto* tag) {
     using OT = std::remove_pointer_t<decltype(tag)>;
     using T8 = std::conditional_t<std::is_same<OT, float>::value, e4m3_wide, e4m3>;
-    rc = args->type == HOTK_E4M3 ? la_product<T8, OT>(*args, workspace, ws_bytes, st)
-                                 : la_product<OT, OT>(*args, workspace, ws_bytes, st);
+      using T8 = std::conditional_t<std::is_same<OT, float>::value, e4m3_wide, e4m3>;
+    rc = args->type == HOTK_E4M3 ? la_product<T8, OT, false, false>(*args, workspace, ws_bytes, st)
+       : args->flags == 0 ? la_product<OT, OT, false, false>(*args, workspace, ws_bytes, st)
+       : args->flags == HOTK_LINEAR_W_DOWN ? la_product<OT, OT, false, true>(*args, workspace, ws_bytes, st)
+                                           : la_product<OT, OT, true, true>(*args, workspace, ws_bytes, st);
   });
   return rc;
 }
 
-extern "C" int hotk_linear_turn(const void* in, int64_t ld_in, const void* save, int act, void* out, int64_t ld_out, void* out_t,
-                                int64_t ld_t, float* partial, int64_t R, int64_t C, int type, void* stream) {
-  HOTK_CHECK_ARG(R >= 0 && C > 0 && ld_in >= C && (!out || ld_out >= C) && (!out_t || ld_t >= R));
+extern "C" int hotk_linear_dz_partials(int64_t R, int64_t* n_partials) {
+  HOTK_CHECK_ARG(n_partials && R >= 0);
+  *n_partials = R ? la_div(R, la_dz_rows(R)) : 0;
+  return HOTK_OK;
+}
+
+extern "C" int hotk_linear_dz(const void* in, int64_t ld_in, const void* save, int act, void* out, int64_t ld_out, float* partial,
+                              int64_t R, int64_t C, int type, void* stream) {
+  HOTK_CHECK_ARG(R >= 0 && C > 0 && ld_in >= C && (!out || ld_out >= C) && (out || partial));
   HOTK_CHECK_ARG(act >= HOTK_ACT_NONE && act <= HOTK_ACT_SILU && (act == HOTK_ACT_NONE || save || R == 0));
-  HOTK_CHECK_ARG(out || out_t || partial);
-  if (!ffn_type_ok(type) && type != HOTK_E4M3) return HOTK_EUNSUPPORTED;
-  HOTK_CHECK_ARG(type != HOTK_E4M3 || (act == HOTK_ACT_NONE && !partial));      // (bytes are copied, not added)
+  if (!ffn_type_ok(type)) return HOTK_EUNSUPPORTED;
+  HOTK_CHECK_ARG(ffn_elem_aligned(in, type) && ffn_elem_aligned(out, type) && ((uintptr_t)save) % (type == HOTK_F32 ? 4 : 2) == 0 &&
+                 ((uintptr_t)partial) % 4 == 0);
   if (R == 0) return HOTK_OK;
   HOTK_CHECK_ARG(in);
-  const int64_t across = la_div(out && ld_out > C ? ld_out : C, 64), down = la_div(out_t && ld_t > R ? ld_t : R, 64);
-  if (across > (1 << 20) || down > (1ll << 30) / across) return HOTK_ETOOLARGE;
-  const dim3 grid((unsigned)(across * down)), block(256);
-  hipStream_t st = (hipStream_t)stream;
-  if (type == HOTK_E4M3)
-    hipLaunchKernelGGL((k_linact_turn<uint8_t, false>), grid, block, 0, st, (const uint8_t*)in, ld_in, save, act, (uint8_t*)out,
-                       ld_out, (uint8_t*)out_t, ld_t, partial, R, C, (unsigned)across);
-  else
-    ffn_dispatch(type, [&](auto* tag) {
-      using T = std::remove_pointer_t<decltype(tag)>;
-      hipLaunchKernelGGL((k_linact_turn<T, true>), grid, block, 0, st, (const T*)in, ld_in, save, act, (T*)out, ld_out, (T*)out_t,
-                         ld_t, partial, R, C, (unsigned)across);
-    });
+  const int64_t pieces = la_div(out ? ld_out : C, 16 / ffn_bytes(type)), rows = la_dz_rows(R), down = la_div(R, rows);
+  int cg_log = 0;
+  while (cg_log < 5 && (1 << cg_log) < pieces) ++cg_log;
+  const int64_t across = la_div(pieces, 1 << cg_log);
+  if (across > (1 << 20) || rows > (1 << 30)) return HOTK_ETOOLARGE;
+  ffn_dispatch(type, [&](auto* tag) {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    hipLaunchKernelGGL(k_linact_dz<T>, dim3((unsigned)(across * down)), dim3(256), 0, (hipStream_t)stream, (const T*)in, ld_in, save, act,
+                       (T*)out, ld_out, partial, R, C, (int)rows, cg_log, (unsigned)across);
+  });
+  return hotk_launch_status();
+}
+
+extern "C" int hotk_pad_rows(const void* in, int64_t ld_in, void* out, int64_t ld_out, int64_t R, int64_t bytes, void* stream) {
+  HOTK_CHECK_ARG(R >= 0 && bytes > 0 && ld_in >= bytes && ld_out >= bytes && ld_out % 16 == 0);
+  if (R == 0) return HOTK_OK;
+  HOTK_CHECK_ARG(in && out && hotk_aligned16(out));
+  hipLaunchKernelGGL(k_pad_rows, dim3(hotk_grid(R * (ld_out / 16), 256)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)in, ld_in,
+                     (uint8_t*)out, ld_out, R, bytes);
   return hotk_launch_status();
 }

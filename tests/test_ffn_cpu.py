@@ -51,7 +51,7 @@ def test_norm_entries_refuse():
 
 def _args(**kw):
     a = dict(M=4, N=8, K=32, x=4096, ld_x=32, w=4096, ld_w=32, bias=0, res=0, ld_res=0, y=4096, ld_y=8, save=0, x_scale=0,
-             w_scale=0, type=1, out_type=1, act=0, reserved=0)
+             w_scale=0, type=1, out_type=1, act=0, flags=0)
     a.update(kw)
     return _lib.LinearArgs(**a)
 
@@ -64,7 +64,9 @@ def _args(**kw):
     ('mixed types', dict(out_type=0), EUNSUPPORTED), ('8 bits without scales', dict(type=3), EINVAL),
     ('scales without 8 bits', dict(x_scale=4096, w_scale=4096), EINVAL), ('one scale', dict(type=3, x_scale=4096), EINVAL),
     ('slope of 8 bits', dict(type=3, x_scale=4096, w_scale=4096, save=4096), EINVAL),
-    ('half a piece', dict(K=28), EUNSUPPORTED), ('row stride', dict(ld_x=36), EUNSUPPORTED), ('w row stride', dict(ld_w=36), EUNSUPPORTED),
+    ('half a piece', dict(K=28, ld_x=28, ld_w=28), EUNSUPPORTED), ('x down alone', dict(flags=1, ld_x=8), EUNSUPPORTED),
+    ('unknown flag', dict(flags=4), EINVAL), ('8 bits down', dict(type=3, x_scale=4096, w_scale=4096, flags=2, ld_w=32), EUNSUPPORTED),
+    ('w columns in no whole pieces', dict(flags=2, N=5, ld_w=5, ld_y=5), EUNSUPPORTED), ('row stride', dict(ld_x=36), EUNSUPPORTED), ('w row stride', dict(ld_w=36), EUNSUPPORTED),
     ('x between pieces', dict(x=4098), EUNSUPPORTED), ('w between pieces', dict(w=4104), EUNSUPPORTED),
     ('y between elements', dict(y=4097), EINVAL), ('bias between elements', dict(bias=4097), EINVAL),
     ('row too long', dict(ld_x=1 << 23), ETOOLARGE)])
@@ -82,10 +84,16 @@ def test_product_entry_empty_and_workspace():
     assert L.hotk_linear_act(ctypes.byref(_args(M=128, N=128, K=65536, ld_x=65536, ld_w=65536, ld_y=128)), SOME, need.value - 1, NULL) == EWORKSPACE
 
 
-def test_turn_entry_refuses():
-    turn = lambda i=SOME, ld=8, save=NULL, act=0, out=SOME, ld_o=8, out_t=NULL, ld_t=0, part=NULL, R=4, C=8, ty=1: L.hotk_linear_turn(
-        i, ld, save, act, out, ld_o, out_t, ld_t, part, R, C, ty, NULL)
-    assert turn(R=0) == 0
-    assert turn(i=NULL) == EINVAL and turn(ld=7) == EINVAL and turn(ld_o=7) == EINVAL and turn(out=NULL) == EINVAL
-    assert turn(out_t=SOME, ld_t=3) == EINVAL and turn(act=3) == EINVAL and turn(act=6, save=SOME) == EINVAL
-    assert turn(ty=5) == EUNSUPPORTED and turn(ty=3, part=SOME) == EINVAL and turn(ty=3, act=1, save=SOME) == EINVAL
+def test_backward_entries_refuse():
+    dz = lambda i=SOME, ld=8, save=NULL, act=0, out=SOME, ld_o=8, part=NULL, R=4, C=8, ty=1: L.hotk_linear_dz(
+        i, ld, save, act, out, ld_o, part, R, C, ty, NULL)
+    assert dz(R=0) == 0
+    assert dz(i=NULL) == EINVAL and dz(ld=7) == EINVAL and dz(ld_o=7) == EINVAL and dz(out=NULL) == EINVAL and dz(C=0, ld=0, ld_o=0) == EINVAL
+    assert dz(act=3) == EINVAL and dz(act=6, save=SOME) == EINVAL and dz(i=ctypes.c_void_p(4097)) == EINVAL
+    assert dz(ty=5) == EUNSUPPORTED and dz(ty=3) == EUNSUPPORTED
+    n = ctypes.c_int64()
+    for R, want in ((0, 0), (1, 1), (64, 1), (65, 2), (65536, 1024), (65537, 513), (10 ** 7, 1022)):
+        assert L.hotk_linear_dz_partials(R, ctypes.byref(n)) == 0 and n.value == want, (R, n.value)
+    pad = lambda i=SOME, ld=8, out=SOME, ld_o=16, R=4, nb=8: L.hotk_pad_rows(i, ld, out, ld_o, R, nb, NULL)
+    assert pad(R=0) == 0 and pad(i=NULL) == EINVAL and pad(ld=7) == EINVAL and pad(ld_o=8) == EINVAL and pad(ld_o=24) == EINVAL
+    assert pad(out=ctypes.c_void_p(4104)) == EINVAL and pad(nb=0) == EINVAL
