@@ -328,9 +328,6 @@ Tensor product(const Rows& x, const Rows& w, int64_t M, int64_t N, int64_t K, at
   const Tensor y = like(x.t, {M, N}, type);
   if (M == 0) return y;
   const int ty = type_of(x.t.scalar_type());
-  size_t need = 0;
-  check(L.linear_workspace_bytes(M, N, K, ty, &need), "hotk_linear_workspace_bytes");
-  const Tensor ws = need ? like(x.t, {(int64_t)need}, at::kByte) : Tensor();
   hotk_linear_args a{};
   a.M = M; a.N = N; a.K = K;
   a.x = x.p(); a.ld_x = x.ld;
@@ -341,6 +338,9 @@ Tensor product(const Rows& x, const Rows& w, int64_t M, int64_t N, int64_t K, at
   a.save = out(e.save);
   a.x_scale = (const float*)out(e.x_scale); a.w_scale = (const float*)out(e.w_scale);
   a.type = ty; a.out_type = type_of(type); a.act = e.act; a.flags = e.flags;
+  size_t need = 0;
+  check(L.linear_workspace_bytes(&a, &need), "hotk_linear_act");
+  const Tensor ws = need ? like(x.t, {(int64_t)need}, at::kByte) : Tensor();
   launch("hotk_linear_act", (M + N) * K * x.t.element_size() + M * N * y.element_size() * (1 + e.res.t.defined()),
          [&] { return L.linear_act(&a, out(ws), need, stream_of(x.t)); });
   return y;

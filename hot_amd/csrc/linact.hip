@@ -22,13 +22,12 @@
 // matrix instructions: by then every fragment of the stage is in registers and the next stage has landed, so behind the
 // barrier the DMA of the step after next starts and the next step's first fragments are read while matrix instructions run.
 //
-// The weight is the matrix instruction's row operand; eight lane-group swaps then give a lane 16 consecutive output columns,
-// so bias, residual, y and the saved slope move in 16-byte accesses without a pass through LDS.
-//
 // For training, 16-bit types keep f'(z) as a 16-bit fixed-point number in steps of 2^-14 (|f'| < 1.13): its error of 2^-15
 // is far below the rounding of dz, where z rounded to the type would add as much as that rounding again, and the backward
 // pass needs no transcendental.  fp32 keeps z.
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "ffn.h"
@@ -160,7 +159,7 @@ __device__ __forceinline__ void la_activate(const LaEpi<OT>& e, int64_t m, int64
   }
 }
 
-// W consecutive columns (a multiple of 8) of one row, from n0: z is the bare product.  The activation is chosen once per piece:
+// W consecutive columns (a multiple of the 16-byte piece) of one row, from n0: z is the bare product.  The activation is chosen once per piece:
 // W independent chains run side by side
 template <int W, class OT>
 __device__ __forceinline__ void la_finish(const LaEpi<OT>& e, int64_t m, int64_t n0, int64_t N, float (&z)[W]) {
@@ -302,25 +301,21 @@ struct LaFrag<e4m3_wide> {
   }
 };
 
+// matrix instructions of one fragment pair, in parts of one instruction each
+template <class IT> struct LaParts { static constexpr int N = 2; };
+template <> struct LaParts<float> { static constexpr int N = 8; };
+template <> struct LaParts<e4m3> { static constexpr int N = 1; };
+template <> struct LaParts<e4m3_wide> { static constexpr int N = 4; };
 template <class IT>
-__device__ __forceinline__ void la_mma(f32x4& c, const LaFrag<IT>& w, const LaFrag<IT>& x) {
+__device__ __forceinline__ void la_mma(int p, f32x4& c, const LaFrag<IT>& w, const LaFrag<IT>& x) {
   if constexpr (std::is_same<IT, __bf16>::value) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w.h[h]), __builtin_bit_cast(bf16x8, x.h[h]), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w.h[p]), __builtin_bit_cast(bf16x8, x.h[p]), c, 0, 0, 0);
   } else if constexpr (std::is_same<IT, _Float16>::value) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w.h[h]), __builtin_bit_cast(f16x8, x.h[h]), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w.h[p]), __builtin_bit_cast(f16x8, x.h[p]), c, 0, 0, 0);
   } else if constexpr (std::is_same<IT, float>::value) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w.h[h][k]), __uint_as_float(x.h[h][k]), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w.h[p >> 2][p & 3]), __uint_as_float(x.h[p >> 2][p & 3]), c, 0, 0, 0);
   } else if constexpr (std::is_same<IT, e4m3_wide>::value) {
-#pragma unroll
-    for (int h = 0; h < 4; ++h) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.b[h], x.b[h], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.b[p], x.b[p], c, 0, 0, 0);
   } else {
     const i32x8 wv = {(int)w.h[0][0], (int)w.h[0][1], (int)w.h[0][2], (int)w.h[0][3], (int)w.h[1][0], (int)w.h[1][1], (int)w.h[1][2], (int)w.h[1][3]};
     const i32x8 xv = {(int)x.h[0][0], (int)x.h[0][1], (int)x.h[0][2], (int)x.h[0][3], (int)x.h[1][0], (int)x.h[1][1], (int)x.h[1][2], (int)x.h[1][3]};
@@ -383,6 +378,8 @@ struct LaFeed {
 template <class IT, class OT, bool TA, bool TB, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void k_linact_tile(const LaTile<OT> g) {
   constexpr int NW = WM * WN, TM = BM / WM, MF = TM / 16, NF = 4, STAGE = (BM + BN) * 128;
+  // (the two x stages side by side where both operands lie along rows: 2 % faster; where one is read across, stage by stage)
+  constexpr int XS = TB ? STAGE : BM * 128, WS = TB ? STAGE : BN * 128, W0 = TB ? BM * 128 : 2 * BM * 128;
   static_assert(BN / WN == 64 && BM % (16 * WM) == 0, "a wave owns 64 columns");
   using SA = LaSide<IT, TA, BM>;
   using SB = LaSide<IT, TB, BN>;
@@ -397,8 +394,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linact_tile(const LaTile<OT> g
   const LaFeed<IT, TA, BM, NW> fa(g.a, g.lda, m0, g.M, wave, lane);
   const LaFeed<IT, TB, BN, NW> fb(g.b, g.ldb, n0, g.N, wave, lane);
   auto issue = [&](int kt, int stage) {
-    fa.issue(kt, g.K, lds0 + stage * STAGE);
-    fb.issue(kt, g.K, lds0 + stage * STAGE + BM * 128);
+    fa.issue(kt, g.K, lds0 + stage * XS);
+    fb.issue(kt, g.K, lds0 + W0 + stage * WS);
   };
 
   f32x4 acc[MF][NF];
@@ -411,11 +408,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linact_tile(const LaTile<OT> g
 #pragma unroll
     for (int j = 0; j < NF; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) f[j].set(h, SB::frag(lds + stage * STAGE + BM * 128, wn * 64 + 16 * j, h, lr, lg));
+      for (int h = 0; h < 2; ++h) f[j].set(h, SB::frag(lds + W0 + stage * WS, wn * 64 + 16 * j, h, lr, lg));
   };
   auto read_x = [&](int stage, int i, LaFrag<IT>& f) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) f.set(h, SA::frag(lds + stage * STAGE, wm * TM + 16 * i, h, lr, lg));
+    for (int h = 0; h < 2; ++h) f.set(h, SA::frag(lds + stage * XS, wm * TM + 16 * i, h, lr, lg));
   };
   // step kt from stage S: fragments 0 are in registers.  Before the last row of matrix instructions the stage has been read
   // whole, and step kt + 1 has landed in the other
@@ -432,8 +429,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linact_tile(const LaTile<OT> g
         read_w(S ^ 1, wf[S ^ 1]);
         read_x(S ^ 1, 0, xf[MF > 1 ? 0 : 1]);
       }
+      __builtin_amdgcn_sched_barrier(0);       // the reads are under way before the matrix instructions that hide them
 #pragma unroll
-      for (int j = 0; j < NF; ++j) la_mma<IT>(acc[i][j], wf[S][j], xf[i & 1]);
+      for (int p = 0; p < LaParts<IT>::N; ++p)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) la_mma<IT>(p, acc[i][j], wf[S][j], xf[i & 1]);
     }
     if (MF == 1) xf[0] = xf[1];
   };
@@ -452,33 +452,49 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linact_tile(const LaTile<OT> g
     }
   }
 
-  const int64_t n = n0 + wn * 64 + 16 * lg;
+  // Out: HALF * 16 rows of the wave at a time go through its own piece of LDS, after which a lane holds V consecutive columns and
+  // neighbouring lanes whole lines of a row.  The activations are a loop over pieces with one copy of the code, kept small:
+  // unrolled over the accumulators it was 40 KB that every tile ran once, and fetching it took longer than running it (a 256 x 256
+  // tile's end: 35 us against 6)
+  constexpr int V = Elem<OT>::VEC, PER_ROW = 64 / V, ROWS = 64 / PER_ROW, PITCH = 68;
+  constexpr int HALF = MF > 4 ? 4 : MF;
+  static_assert(NW * HALF * 16 * PITCH * 4 <= 160 * 1024 && MF % HALF == 0, "the waves' pieces fit LDS");
+  la_barrier();                          // every wave has read the last stage
+  float* box = reinterpret_cast<float*>(lds) + wave * HALF * 16 * PITCH;
+  const int64_t n = n0 + wn * 64 + V * (lane % PER_ROW);
+  const int left = (int)(g.N - n < V ? g.N - n : V);
+#pragma unroll 1
+  for (int half = 0; half < MF / HALF; ++half) {
 #pragma unroll
-  for (int i = 0; i < MF; ++i) {
-    const int64_t m = m0 + wm * TM + 16 * i + lr;
-    // lane group q holds columns 4 q .. of each of the four fragments: swapped so that group q holds the 16 columns of fragment q
-    float z[16];
+    for (int s = 0; s < MF / HALF; ++s)
+      if (s == half) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const auto u02 = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][0][k]), __float_as_uint(acc[i][2][k]), false, false);
-      const auto u13 = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[i][1][k]), __float_as_uint(acc[i][3][k]), false, false);
-      const auto lo = __builtin_amdgcn_permlane16_swap(u02[0], u13[0], false, false);
-      const auto hi = __builtin_amdgcn_permlane16_swap(u02[1], u13[1], false, false);
-      z[k] = __uint_as_float(lo[0]);
-      z[4 + k] = __uint_as_float(lo[1]);
-      z[8 + k] = __uint_as_float(hi[0]);
-      z[12 + k] = __uint_as_float(hi[1]);
+        for (int i = 0; i < HALF; ++i)
+#pragma unroll
+          for (int j = 0; j < NF; ++j) *reinterpret_cast<f32x4*>(box + (16 * i + lr) * PITCH + 16 * j + 4 * lg) = acc[s * HALF + i][j];
+      }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int r = lane / PER_ROW; r < HALF * 16; r += ROWS) {
+      const int64_t m = m0 + wm * TM + half * (HALF * 16) + r;
+      float z[V];
+#pragma unroll
+      for (int k = 0; k < V; k += 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(box + r * PITCH + V * (lane % PER_ROW) + k);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) z[k + q] = v[q];
+      }
+      if (m >= g.M || left <= 0) continue;
+      if (g.part) {
+        float* row = g.part + ((int64_t)blockIdx.y * g.M + m) * g.N + n;
+#pragma unroll
+        for (int k = 0; k < V; k += 4)
+          if (k < left) ffn_store(row, k, left, f32x4{z[k], z[k + 1], z[k + 2], z[k + 3]});
+      } else {
+        la_finish<V>(g.e, m, n, g.N, z);
+      }
     }
-    if (m >= g.M) continue;
-    if (g.part) {
-      float* row = g.part + ((int64_t)blockIdx.y * g.M + m) * g.N + n;
-      const int left = (int)(g.N - n < 16 ? g.N - n : 16);
-#pragma unroll
-      for (int j = 0; j < 16; j += 4)
-        if (j < left) ffn_store(row, j, left, f32x4{z[j], z[j + 1], z[j + 2], z[j + 3]});
-    } else {
-      la_finish<16>(g.e, m, n, g.N, z);
-    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
@@ -501,6 +517,80 @@ __global__ __launch_bounds__(256) void k_linact_join(const float* __restrict__ p
       }
     }
     la_finish<8>(e, m, n, N, z);
+  }
+}
+
+// ---- few rows: a weight read once ----------------------------------------------------------------------------------------
+// 16 columns of the result a workgroup, MB blocks of 16 rows of x; the waves take the contraction's steps in turn, fragments
+// come straight from global memory (U steps of them under way), the waves' sums meet in LDS and are finished there.  One
+// launch where the tile kernel would need a split and a join: 3.5 us against 7.2 at 1 x 4 096 x 1 024 (bf16, 8 MB of weight).
+// Every workgroup reads all of x, so with more rows or a long contraction the tiles win: la_shape.  (64 columns a workgroup
+// were slower but for 16 x 16 384 x 4 096, where the tiles are as fast.)
+template <class IT, class OT, int MB>
+__global__ __launch_bounds__(512) void k_linact_few(const LaTile<OT> g) {
+  constexpr int WAVES = 8, E = LaBytes<IT>::E, V = Elem<OT>::VEC, PITCH = 20;
+  constexpr int U = MB == 1 ? 4 : MB == 2 ? 2 : 1;                 // (registers: 8 U (1 + MB) of them hold pieces under way)
+  __shared__ __align__(16) float sums[WAVES][MB * 16][PITCH];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16, chunks = (g.K * E + 15) / 16;
+  const char* wrow = g.b + (n0 + lr < g.N ? n0 + lr : g.N - 1) * g.ldb;
+  const char* xrow[MB];
+  f32x4 acc[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) {
+    xrow[b] = g.a + (16 * b + lr < g.M ? 16 * b + lr : g.M - 1) * g.lda;
+    acc[b] = 0.f;
+  }
+  auto piece = [&](const char* row, int64_t c) {
+    u32x4 v = 0;
+    if (c < chunks) v = *reinterpret_cast<const u32x4*>(row + c * 16);
+    return v;
+  };
+  for (int k0 = wave; k0 < g.ktiles; k0 += WAVES * U) {
+    u32x4 w[U][2], x[U][MB][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t c = (int64_t)(k0 + u * WAVES) * 8 + 4 * h + lg;
+        w[u][h] = piece(wrow, c);
+#pragma unroll
+        for (int b = 0; b < MB; ++b) x[u][b][h] = piece(xrow[b], c);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      LaFrag<IT> fw, fx[MB];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        fw.set(h, w[u][h]);
+#pragma unroll
+        for (int b = 0; b < MB; ++b) fx[b].set(h, x[u][b][h]);
+      }
+#pragma unroll
+      for (int p = 0; p < LaParts<IT>::N; ++p)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) la_mma<IT>(p, acc[b], fw, fx[b]);
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < MB; ++b) *reinterpret_cast<f32x4*>(&sums[wave][16 * b + lr][4 * lg]) = acc[b];
+  __syncthreads();
+  constexpr int PER_ROW = 16 / V;
+  for (int t = threadIdx.x; t < MB * 16 * PER_ROW; t += 64 * WAVES) {
+    const int m = t / PER_ROW, c = t % PER_ROW * V;
+    if (m >= g.M || n0 + c >= g.N) continue;
+    float z[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) z[k] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+#pragma unroll
+      for (int k = 0; k < V; k += 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(&sums[w][m][c + k]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) z[k + q] += v[q];
+      }
+    la_finish<V>(g.e, m, n0 + c, g.N, z);
   }
 }
 
@@ -583,27 +673,56 @@ __global__ __launch_bounds__(256) void k_pad_rows(const uint8_t* __restrict__ in
 // ---- host --------------------------------------------------------------------------------------------------------------
 int64_t la_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// tile and split of a product
-struct LaShape { int bm, bn, splits; };
-LaShape la_shape(int64_t M, int64_t N, int64_t ktiles) {
-  LaShape s{256, 256, 1};
-  if (la_div(M, 256) * la_div(N, 256) < 192) s = {128, 128, 1};
-  if (la_div(M, 128) * la_div(N, 128) < 128) s = {64, 64, 1};
-  if (M <= 32) s = {32, 128, 1};
-  const int64_t tiles = la_div(M, s.bm) * la_div(N, s.bn);
-  // fewer tiles than compute units: the contraction is split until there is one workgroup each, four steps or more a split
-  if (tiles < 192) {
-    int64_t want = 256 / (tiles < 1 ? 1 : tiles);
-    if (want > ktiles / 4) want = ktiles / 4;
-    if (want > LA_MAX_SPLIT) want = LA_MAX_SPLIT;
-    if (want > 1) s.splits = (int)la_div(ktiles, la_div(ktiles, want));
+// Which kernel, tile and split a product takes: the least of their times by a model of what was measured (us, bf16: 128-byte
+// steps; sweeps of all tiles and splits over M, N of 1 .. 16 384 and K of 256 .. 16 384).  A workgroup's step takes `lat` alone, and
+// `sat` for each of those that share a compute unit where that is more; `end` is its start and end.  The matrix work of a step
+// is 8 times a 16-bit type's in fp32, twice with 8-bit operands and an fp32 result.
+struct LaShape { int bm, bn, splits; };      // bn 16: k_linact_few, bm / 16 blocks of rows
+struct LaCost { int bm, bn; float sat, lat, end; };
+const LaCost LA_COSTS[] = {{256, 256, 1.58f, 1.58f, 6.f}, {128, 128, 0.42f, 0.69f, 3.f}, {64, 64, 0.155f, 0.43f, 0.6f}, {32, 128, 0.175f, 0.32f, 0.7f}};
+LaShape la_shape(int64_t M, int64_t N, int64_t K, int type, int out_type, int flags) {
+  const int64_t ktiles = la_div(K * ffn_bytes(type), 128);
+  const bool wide = type == HOTK_E4M3 && out_type == HOTK_F32;
+  const float mfma = type == HOTK_F32 ? 8.f : wide ? 2.f : 1.f;
+  LaShape best{64, 64, 1};
+  float least = 1e30f;
+  if (M <= 64 && flags == 0) {               // k_linact_few: 8.6 TB/s in all, 50 GB/s a compute unit, its matrix work beside that
+    const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    const float wgs = (float)la_div(N, 16), bytes = ktiles * 128.f * 16 * (1 + mb);
+    least = std::max(std::max(wgs * bytes / 8.6e6f, std::ceil(wgs / 256.f) * bytes / 50e3f),
+                     std::ceil(wgs / 256.f) * ktiles * 0.89f * mfma * mb / 256.f);
+    best = {16 * mb, 16, 1};
   }
-  return s;
+  for (const LaCost& c : LA_COSTS) {
+    // (256 x 256 spills registers with bf16 copies of 8-bit operands; with both operands transposed a step takes 3.7)
+    if (c.bm == 256 && wide) continue;
+    const float flop = 0.89f * mfma * (c.bm * c.bn) / 65536.f;              // a step's matrix work at the clock's rate
+    const float sat = std::max(c.bm == 256 && flags == (HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN) ? 3.7f : c.sat, 1.05f * flop);
+    const double tiles = (double)la_div(M, c.bm) * la_div(N, c.bn);
+    for (int64_t s = 1; s <= LA_MAX_SPLIT && s <= ktiles; s *= 2) {
+      const int64_t kper = la_div(ktiles, s), splits = la_div(ktiles, kper);
+      const float q = (float)std::ceil(tiles * splits / 256.);
+      float t = q * c.end + kper * std::max(std::max(c.lat, flop), sat * q);
+      if (splits > 1) t += 3.5f + splits * (float)M * N * 4.f / 3e6f;       // the join: a launch, and the parts written and read
+      if (t < least) {
+        least = t;
+        best = {c.bm, c.bn, (int)splits};
+      }
+    }
+  }
+  return best;
+}
+
+template <class IT, class OT, int MB>
+int la_run_few(const LaTile<OT>& g, hipStream_t st) {
+  hipLaunchKernelGGL((k_linact_few<IT, OT, MB>), dim3((unsigned)la_div(g.N, 16)), dim3(512), 0, st, g);
+  return hotk_launch_status();
 }
 
 template <class IT, class OT, bool TA, bool TB, int BM, int BN, int WM, int WN>
 int la_run(LaTile<OT>& g, int splits, hipStream_t st) {
-  constexpr int LDS = 2 * (BM + BN) * 128;
+  // two stages, or the waves' pieces of the result where those are larger
+  constexpr int BOX = WM * WN * (BM / WM < 64 ? BM / WM : 64) * 68 * 4, STAGES = 2 * (BM + BN) * 128, LDS = BOX > STAGES ? BOX : STAGES;
   auto kernel = k_linact_tile<IT, OT, TA, TB, BM, BN, WM, WN>;
   if (LDS > 64 * 1024) {                 // more LDS than a kernel gets without asking: asked for once per device
     static std::atomic<uint64_t> asked{0};
@@ -625,7 +744,7 @@ template <class IT, class OT, bool TA, bool TB>
 int la_product(const hotk_linear_args& a, void* ws, size_t nws, hipStream_t st) {
   const int e = ffn_bytes(a.type);
   const int64_t ktiles = la_div(a.K * e, 128);
-  const LaShape s = la_shape(a.M, a.N, ktiles);
+  const LaShape s = la_shape(a.M, a.N, a.K, a.type, a.out_type, a.flags);
   const size_t need = s.splits > 1 ? (size_t)s.splits * a.M * a.N * 4 : 0;
   if (nws < need || (need && !ws)) return HOTK_EWORKSPACE;
   LaTile<OT> g{};
@@ -635,6 +754,8 @@ int la_product(const hotk_linear_args& a, void* ws, size_t nws, hipStream_t st) 
   g.ktiles = (int)ktiles; g.kper = (int)la_div(ktiles, s.splits);
   g.part = need ? (float*)ws : nullptr;
   g.e = {(const OT*)a.bias, (const OT*)a.res, a.ld_res, (OT*)a.y, a.ld_y, a.save, a.x_scale, a.w_scale, a.act};
+  if constexpr (!TA && !TB)
+    if (s.bn == 16) return s.bm == 16 ? la_run_few<IT, OT, 1>(g, st) : s.bm == 32 ? la_run_few<IT, OT, 2>(g, st) : la_run_few<IT, OT, 4>(g, st);
   int rc = s.bm == 256 ? la_run<IT, OT, TA, TB, 256, 256, 2, 4>(g, s.splits, st)
          : s.bm == 128 ? la_run<IT, OT, TA, TB, 128, 128, 2, 2>(g, s.splits, st)
          : s.bm == 64 ? la_run<IT, OT, TA, TB, 64, 64, 2, 1>(g, s.splits, st)
@@ -679,11 +800,11 @@ int64_t la_dz_rows(int64_t R) { return la_div(la_div(R, 1024), 64) * 64; }
 
 }  // namespace
 
-extern "C" int hotk_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int type, size_t* bytes) {
-  HOTK_CHECK_ARG(bytes && M >= 0 && N > 0 && K > 0);
-  if (!(ffn_type_ok(type) || type == HOTK_E4M3)) return HOTK_EUNSUPPORTED;
-  const LaShape s = la_shape(M, N, la_div(K * ffn_bytes(type), 128));
-  *bytes = s.splits > 1 ? (size_t)s.splits * M * N * 4 : 0;
+extern "C" int hotk_linear_workspace_bytes(const hotk_linear_args* args, size_t* bytes) {
+  HOTK_CHECK_ARG(args && bytes);
+  if (const int rc = la_check(*args)) return rc;
+  const LaShape s = la_shape(args->M, args->N, args->K, args->type, args->out_type, args->flags);
+  *bytes = s.splits > 1 ? (size_t)s.splits * args->M * args->N * 4 : 0;
   return HOTK_OK;
 }
 

@@ -278,25 +278,24 @@ __global__ __launch_bounds__(64 * WAVES) void k_rmsnorm_bwd(const RnBwd<T> a) {
   }
 }
 
-// out[c] = sum over b of partial[b][c], in an order that the sizes alone set: a wave adds every 16th row, the sixteen are
-// joined in order
-constexpr int SP_WAVES = 16;
+// out[c] = sum over b of partial[b][c], in an order that the sizes alone set: 16 columns a workgroup, its 64 row lanes add every
+// 64th row each (eight loads under way), LDS joins them by halves
 template <class T>
-__global__ __launch_bounds__(64 * SP_WAVES) void k_sum_partials(const float* __restrict__ partial, int64_t n, int64_t D,
-                                                                T* __restrict__ out) {
-  __shared__ float part[SP_WAVES][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+__global__ __launch_bounds__(1024) void k_sum_partials(const float* __restrict__ partial, int64_t n, int64_t D, T* __restrict__ out) {
+  __shared__ float part[64][17];
+  const int col = threadIdx.x & 15, row = threadIdx.x >> 4;
+  const int64_t c = (int64_t)blockIdx.x * 16 + col;
   float s = 0.f;
-  if (c < D)
-    for (int64_t b = wave; b < n; b += SP_WAVES) s += partial[b * D + c];
-  part[wave][lane] = s;
-  __syncthreads();
-  if (wave == 0 && c < D) {
-#pragma unroll
-    for (int w = 1; w < SP_WAVES; ++w) s += part[w][lane];
-    out[c] = (T)s;
+  if (c < D) {
+#pragma unroll 8
+    for (int64_t b = row; b < n; b += 64) s += partial[b * D + c];
   }
+  part[row][col] = s;
+  for (int half = 32; half >= 1; half >>= 1) {
+    __syncthreads();
+    if (row < half) part[row][col] += part[row + half][col];
+  }
+  if (row == 0 && c < D) out[c] = (T)part[0][col];
 }
 
 unsigned rn_grid(int64_t rows, int groups, unsigned cap) {
@@ -442,7 +441,7 @@ extern "C" int hotk_sum_partials(const float* partial, int64_t n, int64_t D, voi
   if (!ffn_type_ok(type)) return HOTK_EUNSUPPORTED;
   if (D == 0) return HOTK_OK;
   HOTK_CHECK_ARG(out && (partial || n == 0) && ffn_elem_aligned(out, type));
-  const dim3 grid((unsigned)((D + 63) / 64)), block(64 * SP_WAVES);
+  const dim3 grid((unsigned)((D + 15) / 16)), block(1024);
   ffn_dispatch(type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     hipLaunchKernelGGL(k_sum_partials<T>, grid, block, 0, (hipStream_t)stream, partial, n, D, (T*)out);

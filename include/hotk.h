@@ -556,7 +556,7 @@ typedef struct {
   const float* w_scale;
   int32_t type, out_type, act, flags;
 } hotk_linear_args;
-int hotk_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int type, size_t* bytes);
+int hotk_linear_workspace_bytes(const hotk_linear_args* args, size_t* bytes);       /* for exactly these arguments */
 int hotk_linear_act(const hotk_linear_args* args, void* workspace, size_t ws_bytes, void* stream);
 /* v = in [R, C] times the slope that `save` holds (HOTK_ACT_NONE: times one); out (NULL: none) [R, ld_out], with zeros from C on;
  * partial (NULL: none) [n][C], n = hotk_linear_dz_partials(R): column sums of v in 32 bits, for hotk_sum_partials */

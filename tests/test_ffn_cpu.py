@@ -78,10 +78,13 @@ def test_product_entry_empty_and_workspace():
     assert L.hotk_linear_act(ctypes.byref(_args(M=0, x=0, w=0, y=0)), NULL, 0, NULL) == 0
     assert L.hotk_linear_act(None, NULL, 0, NULL) == EINVAL
     need = ctypes.c_size_t()
-    assert L.hotk_linear_workspace_bytes(4, 8, 0, 1, ctypes.byref(need)) == EINVAL
-    assert L.hotk_linear_workspace_bytes(128, 128, 65536, 1, ctypes.byref(need)) == 0 and need.value > 0      # few tiles, long contraction
-    assert L.hotk_linear_act(ctypes.byref(_args(M=128, N=128, K=65536, ld_x=65536, ld_w=65536, ld_y=128)), NULL, 0, NULL) == EWORKSPACE
-    assert L.hotk_linear_act(ctypes.byref(_args(M=128, N=128, K=65536, ld_x=65536, ld_w=65536, ld_y=128)), SOME, need.value - 1, NULL) == EWORKSPACE
+    assert L.hotk_linear_workspace_bytes(ctypes.byref(_args(K=0, ld_x=0)), ctypes.byref(need)) == EINVAL
+    long = dict(M=128, N=128, K=65536, ld_x=65536, ld_w=65536, ld_y=128)                         # few tiles, a long contraction
+    assert L.hotk_linear_workspace_bytes(ctypes.byref(_args(**long)), ctypes.byref(need)) == 0 and need.value > 0
+    assert L.hotk_linear_act(ctypes.byref(_args(**long)), NULL, 0, NULL) == EWORKSPACE
+    assert L.hotk_linear_act(ctypes.byref(_args(**long)), NULL, need.value, NULL) == EWORKSPACE
+    assert L.hotk_linear_act(ctypes.byref(_args(**long)), SOME, need.value - 1, NULL) == EWORKSPACE
+    assert L.hotk_linear_workspace_bytes(ctypes.byref(_args()), ctypes.byref(need)) == 0 and need.value == 0
 
 
 def test_backward_entries_refuse():
