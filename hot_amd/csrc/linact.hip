@@ -56,12 +56,11 @@ template <int ACT, bool FAST>
 __device__ __forceinline__ float la_act(float z, float neg, float& slope) {
   if constexpr (ACT == HOTK_ACT_GELU) {
     float cdf, pdf;
-    if (FAST) {
-      const float x = fabsf(z) * 0.70710678f;
-      const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
-      const float e = __builtin_amdgcn_exp2f(-1.44269504f * x * x);
-      const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * e;
-      cdf = z < 0.f ? 0.5f * q : fmaf(-0.5f, q, 1.f);
+    if (FAST) {            // q = half of erfc(|z| / sqrt 2), cdf = 1/2 + sign(z) (1/2 - q)
+      const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
+      const float e = __builtin_amdgcn_exp2f(z * (-0.72134752f * z));
+      const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f) * e;
+      cdf = 0.5f + copysignf(0.5f - q, z);
       pdf = 0.39894228f * e;
     } else {
       cdf = 0.5f * erfcf(-0.70710678f * z);
@@ -104,9 +103,24 @@ __device__ __forceinline__ float la_act_grad(float z, int act) {
   }
   return d;
 }
-__device__ __forceinline__ int16_t la_slope_code(float d) {
-  const int c = (int)rintf(d * (1.f / LA_SLOPE_STEP));
-  return (int16_t)(d != d ? LA_SLOPE_NAN : c);
+// eight slopes in steps of 2^-14 (the packed conversion's unit is 1 / 32767); a NaN among them is rare, and looked for in their sum
+typedef int16_t s16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ s16x8 la_slope_codes(const float* d) {
+  constexpr float UNIT = 16384.f / 32767.f;
+  s16x8 c;
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) {
+    const auto p = __builtin_amdgcn_cvt_pknorm_i16(d[k] * UNIT, d[k + 1] * UNIT);
+    c[k] = p[0];
+    c[k + 1] = p[1];
+    sum += d[k] + d[k + 1];
+  }
+  if (sum != sum) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) c[k] = d[k] != d[k] ? (int16_t)LA_SLOPE_NAN : c[k];
+  }
+  return c;
 }
 __device__ __forceinline__ float la_slope(int16_t code, int act) {
   if (act == HOTK_ACT_LEAKYRELU) return code > 8192 ? 1.f : LA_LEAK;
@@ -140,14 +154,11 @@ __device__ __forceinline__ void la_activate(const LaEpi<OT>& e, int64_t m, int64
 #pragma unroll
   for (int i = 0; i < W; ++i) z[i] = la_act<ACT, FAST>(z[i], neg, d[i]);
   if (FAST && e.save && e.act != HOTK_ACT_NONE) {
-    typedef int16_t s16x8 __attribute__((ext_vector_type(8)));
     typedef int16_t s16x8u __attribute__((ext_vector_type(8), aligned(2)));
     int16_t* row = (int16_t*)e.save + m * N + n0;
 #pragma unroll
     for (int i = 0; i < W; i += 8) {
-      s16x8 c;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) c[k] = la_slope_code(d[i + k]);
+      const s16x8 c = la_slope_codes(d + i);
       if (i + 8 <= left) {
         *reinterpret_cast<s16x8u*>(row + i) = c;
       } else {
@@ -679,7 +690,7 @@ int64_t la_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // is 8 times a 16-bit type's in fp32, twice with 8-bit operands and an fp32 result.
 struct LaShape { int bm, bn, splits; };      // bn 16: k_linact_few, bm / 16 blocks of rows
 struct LaCost { int bm, bn; float sat, lat, end; };
-const LaCost LA_COSTS[] = {{256, 256, 1.58f, 1.58f, 6.f}, {128, 128, 0.42f, 0.69f, 3.f}, {64, 64, 0.155f, 0.43f, 0.6f}, {32, 128, 0.175f, 0.32f, 0.7f}};
+const LaCost LA_COSTS[] = {{256, 256, 1.58f, 1.58f, 6.f}, {128, 128, 0.42f, 0.69f, 3.f}, {64, 128, 0.26f, 0.39f, 1.2f}, {64, 64, 0.16f, 0.32f, 0.7f}};
 LaShape la_shape(int64_t M, int64_t N, int64_t K, int type, int out_type, int flags) {
   const int64_t ktiles = la_div(K * ffn_bytes(type), 128);
   const bool wide = type == HOTK_E4M3 && out_type == HOTK_F32;
@@ -697,12 +708,13 @@ LaShape la_shape(int64_t M, int64_t N, int64_t K, int type, int out_type, int fl
     // (256 x 256 spills registers with bf16 copies of 8-bit operands; with both operands transposed a step takes 3.7)
     if (c.bm == 256 && wide) continue;
     const float flop = 0.89f * mfma * (c.bm * c.bn) / 65536.f;              // a step's matrix work at the clock's rate
-    const float sat = std::max(c.bm == 256 && flags == (HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN) ? 3.7f : c.sat, 1.05f * flop);
+    const float sat = std::max(c.bm == 256 && flags == (HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN) ? 3.7f : c.sat, 1.12f * flop);
+    const float lat = mfma > 1.f ? c.lat + 0.9f * flop : c.lat;
     const double tiles = (double)la_div(M, c.bm) * la_div(N, c.bn);
     for (int64_t s = 1; s <= LA_MAX_SPLIT && s <= ktiles; s *= 2) {
       const int64_t kper = la_div(ktiles, s), splits = la_div(ktiles, kper);
       const float q = (float)std::ceil(tiles * splits / 256.);
-      float t = q * c.end + kper * std::max(std::max(c.lat, flop), sat * q);
+      float t = q * c.end + kper * std::max(lat, sat * q);
       if (splits > 1) t += 3.5f + splits * (float)M * N * 4.f / 3e6f;       // the join: a launch, and the parts written and read
       if (t < least) {
         least = t;
@@ -758,8 +770,8 @@ int la_product(const hotk_linear_args& a, void* ws, size_t nws, hipStream_t st) 
     if (s.bn == 16) return s.bm == 16 ? la_run_few<IT, OT, 1>(g, st) : s.bm == 32 ? la_run_few<IT, OT, 2>(g, st) : la_run_few<IT, OT, 4>(g, st);
   int rc = s.bm == 256 ? la_run<IT, OT, TA, TB, 256, 256, 2, 4>(g, s.splits, st)
          : s.bm == 128 ? la_run<IT, OT, TA, TB, 128, 128, 2, 2>(g, s.splits, st)
-         : s.bm == 64 ? la_run<IT, OT, TA, TB, 64, 64, 2, 1>(g, s.splits, st)
-                      : la_run<IT, OT, TA, TB, 32, 128, 2, 2>(g, s.splits, st);
+         : s.bn == 128 ? la_run<IT, OT, TA, TB, 64, 128, 2, 2>(g, s.splits, st)
+                       : la_run<IT, OT, TA, TB, 64, 64, 4, 1>(g, s.splits, st);
   if (rc == HOTK_OK && need) {
     const int64_t work = a.M * la_div(a.N, 8);
     hipLaunchKernelGGL(k_linact_join<OT>, dim3(hotk_grid(work, 256)), dim3(256), 0, st, (const float*)ws, s.splits, a.M, a.N, g.e);
@@ -790,7 +802,7 @@ int la_check(const hotk_linear_args& a) {
     HOTK_CHECK_ARG(((uintptr_t)a.x_scale) % 4 == 0 && ((uintptr_t)a.w_scale) % 4 == 0);
   }
   // 32-bit offsets inside a tile, 32-bit tile and step counts
-  if (a.ld_x * e > (1 << 23) || a.ld_w * e > (1 << 23) || la_div(a.M, 32) * la_div(a.N, 64) > (1ll << 30) || la_div(a.K * e, 128) > (1ll << 30))
+  if (a.ld_x * e > (1 << 23) || a.ld_w * e > (1 << 23) || la_div(a.M, 64) * la_div(a.N, 64) > (1ll << 30) || la_div(a.N, 16) > (1ll << 30) || la_div(a.K * e, 128) > (1ll << 30))
     return HOTK_ETOOLARGE;
   return HOTK_OK;
 }

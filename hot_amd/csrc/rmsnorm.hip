@@ -10,8 +10,8 @@
 // Everything between the load and the one rounding at the store is in 32 bits; the norm reads the ROUNDED h, so that the
 // backward pass, which finds h and not x and r, differentiates what the forward pass computed.
 //
-// A group of WPR waves owns a row and holds it in registers, VEC elements (16 bytes) a lane and NV of them, so a row is read
-// once.  Sums cross lanes by shuffles and waves through LDS.  HBM-bound.  A row that is no multiple of VEC has no tail: the
+// A group of LPR lanes (8 to 64 of a wave, or 4, 8 or 16 waves) owns a row and holds it in registers, VEC elements (16 bytes) a
+// lane and NV of them, so a row is read once.  Sums cross lanes by shuffles and waves through LDS.  HBM-bound.  A row that is no multiple of VEC has no tail: the
 // last piece starts VEC before its end, overlapping its neighbour (and so do the lanes past the end); the sums count each
 // element in one lane only, the stores write the same values twice.  Rows shorter than VEC go element by element (SMALL).
 #include "ffn.h"
@@ -22,43 +22,45 @@ constexpr int RN_MAX_D = 32768;
 constexpr float RN_E4M3_MAX = 448.f;
 constexpr float RN_SCALE_MIN = 0x1p-126f;
 
-__device__ __forceinline__ float rn_wave_sum(float v) {
+template <int N>
+__device__ __forceinline__ float rn_lane_sum(float v) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  for (int o = N / 2; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
 // the largest magnitude as the bits of a non-negative float: integer order is float order there, and a NaN is above infinity
-__device__ __forceinline__ uint32_t rn_wave_max(uint32_t v) {
+template <int N>
+__device__ __forceinline__ uint32_t rn_lane_max(uint32_t v) {
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
+  for (int o = N / 2; o >= 1; o >>= 1) {
     const uint32_t t = (uint32_t)__shfl_xor((int)v, o, 64);
     v = t > v ? t : v;
   }
   return v;
 }
-// over the WPR waves of a row's group.  `slot` alternates between calls: one barrier per call is enough, since a wave that
+// over the LPR lanes of a row's group.  `slot` alternates between calls: one barrier per call is enough, since a wave that
 // writes a slot again has passed the barrier of the call in between, which every reader reached after its reads.
-template <int WPR>
-__device__ __forceinline__ float rn_group_sum(float v, float (*box)[16], int& slot, int w) {
-  v = rn_wave_sum(v);
-  if (WPR == 1) return v;
-  if ((threadIdx.x & 63) == 0) box[slot][w] = v;
+template <int LPR>
+__device__ __forceinline__ float rn_group_sum(float v, float (*box)[16], int& slot) {
+  if (LPR <= 64) return rn_lane_sum<LPR>(v);
+  v = rn_lane_sum<64>(v);
+  if ((threadIdx.x & 63) == 0) box[slot][threadIdx.x >> 6] = v;
   __syncthreads();
   float t = 0.f;
 #pragma unroll
-  for (int i = 0; i < WPR; ++i) t += box[slot][i];
+  for (int i = 0; i < LPR / 64; ++i) t += box[slot][i];
   slot ^= 1;
   return t;
 }
-template <int WPR>
-__device__ __forceinline__ uint32_t rn_group_max(uint32_t v, float (*box)[16], int& slot, int w) {
-  v = rn_wave_max(v);
-  if (WPR == 1) return v;
-  if ((threadIdx.x & 63) == 0) box[slot][w] = __uint_as_float(v);
+template <int LPR>
+__device__ __forceinline__ uint32_t rn_group_max(uint32_t v, float (*box)[16], int& slot) {
+  if (LPR <= 64) return rn_lane_max<LPR>(v);
+  v = rn_lane_max<64>(v);
+  if ((threadIdx.x & 63) == 0) box[slot][threadIdx.x >> 6] = __uint_as_float(v);
   __syncthreads();
   uint32_t t = 0;
 #pragma unroll
-  for (int i = 0; i < WPR; ++i) {
+  for (int i = 0; i < LPR / 64; ++i) {
     const uint32_t u = __float_as_uint(box[slot][i]);
     t = u > t ? u : t;
   }
@@ -130,27 +132,25 @@ struct RnFwd {
 
 enum { RN_NORM = 0, RN_NORM8 = 1, RN_QUANT = 2 };
 
-template <class T, int MODE, int NV, int WPR, int WAVES, bool SMALL>
-__global__ __launch_bounds__(64 * WAVES) void k_rmsnorm_fwd(const RnFwd<T> a) {
+// 256 threads a workgroup, or the LPR of one row where that is more (its barriers are then the whole workgroup's)
+template <class T, int MODE, int NV, int LPR, bool SMALL>
+__global__ __launch_bounds__(LPR > 64 ? LPR : 256) void k_rmsnorm_fwd(const RnFwd<T> a) {
   using E = Elem<T>;
   using FV = typename E::fvec;
-  constexpr int VEC = E::VEC, GROUPS = WAVES / WPR, LANES = 64 * WPR;
-  static_assert(WPR == 1 || GROUPS == 1, "a row's group is one wave or the whole workgroup (barriers)");
+  constexpr int VEC = E::VEC, GROUPS = LPR > 64 ? 1 : 256 / LPR;
   __shared__ float box[2][16];
   int slot = 0;
-  const int wave = threadIdx.x >> 6;
-  const int t = WPR == 1 ? (threadIdx.x & 63) : threadIdx.x;
-  const int D = a.D;
-  for (int64_t row = (int64_t)blockIdx.x * GROUPS + (WPR == 1 ? wave : 0); row < a.R; row += (int64_t)gridDim.x * GROUPS) {
+  const int t = threadIdx.x % LPR, D = a.D;
+  for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LPR; row < a.R; row += (int64_t)gridDim.x * GROUPS) {
     const bool kept = !a.kind || hotk_keep(a.keep, a.kind[row]);
     FV v[NV];
     if (kept) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) v[i] = Piece<T, SMALL>(t + LANES * i, D).load(a.x + row * a.ld_x, D);
+      for (int i = 0; i < NV; ++i) v[i] = Piece<T, SMALL>(t + LPR * i, D).load(a.x + row * a.ld_x, D);
       if (MODE != RN_QUANT && a.r) {
         FV r[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) r[i] = Piece<T, SMALL>(t + LANES * i, D).load(a.r + row * a.ld_r, D);
+        for (int i = 0; i < NV; ++i) r[i] = Piece<T, SMALL>(t + LPR * i, D).load(a.r + row * a.ld_r, D);
 #pragma unroll
         for (int i = 0; i < NV; ++i)      // what the norm reads is what is stored
           v[i] = __builtin_convertvector(__builtin_convertvector(v[i] + r[i], typename E::vec), FV);
@@ -163,16 +163,16 @@ __global__ __launch_bounds__(64 * WAVES) void k_rmsnorm_fwd(const RnFwd<T> a) {
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const Piece<T, SMALL> p(t + LANES * i, D);
+        const Piece<T, SMALL> p(t + LPR * i, D);
         if (a.r) p.store(a.h + row * D, D, v[i]);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) s += p.mine(k, D) ? v[i][k] * v[i][k] : 0.f;
       }
-      const float rstd = rsqrtf(rn_group_sum<WPR>(s, box, slot, wave) / (float)D + a.eps);
+      const float rstd = rsqrtf(rn_group_sum<LPR>(s, box, slot) / (float)D + a.eps);
       if (a.rstd && t == 0) a.rstd[row] = rstd;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const Piece<T, SMALL> p(t + LANES * i, D);
+        const Piece<T, SMALL> p(t + LPR * i, D);
         v[i] = v[i] * rstd * p.load(a.w, D);
         if (!kept) v[i] = 0.f;            // (an infinite weight times zero)
         if (MODE == RN_NORM) p.store(a.y + row * D, D, v[i]);
@@ -187,11 +187,11 @@ __global__ __launch_bounds__(64 * WAVES) void k_rmsnorm_fwd(const RnFwd<T> a) {
           const uint32_t u = __float_as_uint(v[i][k]) & 0x7fffffffu;
           m = u > m ? u : m;
         }
-      float scale = __uint_as_float(rn_group_max<WPR>(m, box, slot, wave)) / RN_E4M3_MAX;
+      float scale = __uint_as_float(rn_group_max<LPR>(m, box, slot)) / RN_E4M3_MAX;
       scale = scale < RN_SCALE_MIN ? RN_SCALE_MIN : scale;     // (a NaN stays one)
       if (t == 0) a.scale[row] = scale;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) Piece<T, SMALL>(t + LANES * i, D).store8(a.q + row * D, D, v[i] / scale);
+      for (int i = 0; i < NV; ++i) Piece<T, SMALL>(t + LPR * i, D).store8(a.q + row * D, D, v[i] / scale);
     }
   }
 }
@@ -209,68 +209,68 @@ struct RnBwd {
   int D;
 };
 
-template <class T, int NV, int WPR, int WAVES, bool SMALL>
-__global__ __launch_bounds__(64 * WAVES) void k_rmsnorm_bwd(const RnBwd<T> a) {
+template <class T, int NV, int LPR, bool SMALL>
+__global__ __launch_bounds__(LPR > 64 ? LPR : 256) void k_rmsnorm_bwd(const RnBwd<T> a) {
   using E = Elem<T>;
   using FV = typename E::fvec;
-  constexpr int VEC = E::VEC, GROUPS = WAVES / WPR, LANES = 64 * WPR;
-  static_assert(WPR == 1 || GROUPS == 1, "a row's group is one wave or the whole workgroup (barriers)");
+  constexpr int VEC = E::VEC, GROUPS = LPR > 64 ? 1 : 256 / LPR;
   __shared__ float box[2][16];
-  __shared__ FV fold[GROUPS][64];
+  __shared__ FV fold[GROUPS > 1 ? 4 : 1][64];
   int slot = 0;
-  const int wave = threadIdx.x >> 6;
-  const int t = WPR == 1 ? (threadIdx.x & 63) : threadIdx.x;
-  const int D = a.D;
+  const int t = threadIdx.x % LPR, D = a.D;
   const float inv_d = 1.f / (float)D;
   FV dw[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) dw[i] = 0.f;
-  for (int64_t row = (int64_t)blockIdx.x * GROUPS + (WPR == 1 ? wave : 0); row < a.R; row += (int64_t)gridDim.x * GROUPS) {
+  for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LPR; row < a.R; row += (int64_t)gridDim.x * GROUPS) {
     if (a.kind && !hotk_keep(a.keep, a.kind[row])) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) Piece<T, SMALL>(t + LANES * i, D).store(a.dx + row * D, D, (FV)0.f);
+      for (int i = 0; i < NV; ++i) Piece<T, SMALL>(t + LPR * i, D).store(a.dx + row * D, D, (FV)0.f);
       continue;
     }
     const float rstd = a.rstd[row];
-    FV g[NV], u[NV];
+    FV g[NV], u[NV], o[NV];
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const Piece<T, SMALL> p(t + LANES * i, D);
+      const Piece<T, SMALL> p(t + LPR * i, D);
       g[i] = p.load(a.dy + row * a.ld_dy, D);
       u[i] = p.load(a.h + row * a.ld_h, D);
+      o[i] = a.dh ? p.load(a.dh + row * a.ld_dh, D) : (FV)0.f;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const Piece<T, SMALL> p(t + LANES * i, D);
+      const Piece<T, SMALL> p(t + LPR * i, D);
       u[i] *= rstd;
       dw[i] += g[i] * u[i];
       g[i] *= p.load(a.w, D);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) s += p.mine(k, D) ? g[i][k] * u[i][k] : 0.f;
     }
-    const float m = rn_group_sum<WPR>(s, box, slot, wave) * inv_d;
+    const float m = rn_group_sum<LPR>(s, box, slot) * inv_d;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const Piece<T, SMALL> p(t + LANES * i, D);
-      FV o = rstd * (g[i] - u[i] * m);
-      if (a.dh) o += p.load(a.dh + row * a.ld_dh, D);
-      p.store(a.dx + row * D, D, o);
+      const Piece<T, SMALL> p(t + LPR * i, D);
+      p.store(a.dx + row * D, D, o[i] + rstd * (g[i] - u[i] * m));
     }
   }
-  // one partial row of dw per workgroup: a group's lanes own their columns, the waves of WPR = 1 are added in wave order
+  // one partial row of dw per workgroup: rows side by side in a wave are added across lanes, the waves in order through LDS
   float* out = a.partial + (int64_t)blockIdx.x * D;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const Piece<T, SMALL> p(t + LANES * i, D);
+    const Piece<T, SMALL> p(t + LPR * i, D);
     FV o = dw[i];
     if (GROUPS > 1) {
-      __syncthreads();
-      fold[wave][t] = o;
-      __syncthreads();
-      if (wave != 0) continue;
 #pragma unroll
-      for (int w = 1; w < GROUPS; ++w) o += fold[w][t];
+      for (int k = 0; k < VEC; ++k)
+#pragma unroll
+        for (int d = 32; d >= LPR; d >>= 1) o[k] += __shfl_xor(o[k], d, 64);
+      __syncthreads();
+      fold[threadIdx.x >> 6][threadIdx.x & 63] = o;
+      __syncthreads();
+      if (threadIdx.x >= LPR) continue;
+#pragma unroll
+      for (int w = 1; w < 4; ++w) o += fold[w][t];
     }
 #pragma unroll
     for (int k = 0; k < VEC; ++k)
@@ -303,53 +303,72 @@ unsigned rn_grid(int64_t rows, int groups, unsigned cap) {
   return (unsigned)(g < 1 ? 1 : (g > cap ? cap : g));
 }
 
-// (waves per row, pieces per lane) for a row of D: one wave up to four pieces a lane, then a workgroup of 4 or 16
-struct RnShape { int wpr, nv; };
-RnShape rn_shape(int64_t D, int vec) {
-  if (D < vec) return {0, 0};                       // SMALL
-  const int64_t vecs = (D + vec - 1) / vec;
-  for (int wpr : {1, 4, 16})
-    for (int nv : {1, 2, 4})
-      if (vecs <= 64ll * wpr * nv) return {wpr, nv};
-  return {16, 8};
+// lanes per row and pieces per lane for a row of D: as few lanes as hold it in one or two pieces.  Measured at 16 384 rows of 4 096
+// bf16: the norm with a residual 93 us with 8 waves and one piece, 94 / 98 with 4 and two / four, its backward pass 98 / 102 / 124;
+// rows to 8 bits, with two sums to wait for and less to move, 48 / 38 / 43, so there a lane holds more.
+struct RnShape { int lpr, nv; };
+RnShape rn_shape(int64_t D, int vec, bool quant) {
+  if (D < vec) return {8, 0};                       // SMALL
+  const int64_t v = (D + vec - 1) / vec;
+  if (v <= 64) return {v <= 8 ? 8 : v <= 16 ? 16 : v <= 32 ? 32 : 64, 1};
+  if (v <= 128) return {64, 2};
+  if (v <= 256) return quant ? RnShape{64, 4} : RnShape{256, 1};
+  if (v <= 512) return quant ? RnShape{256, 2} : RnShape{512, 1};
+  if (v <= 1024) return quant ? RnShape{256, 4} : RnShape{512, 2};
+  return {1024, v <= 2048 ? 2 : v <= 4096 ? 4 : 8};
 }
-
-// RUN(pieces, waves per row, waves per workgroup, SMALL)
-#define RN_PICK(RUN)                                     \
-  switch (sh.wpr * 16 + sh.nv) {                         \
-    case 0: RUN(1, 1, 4, true); break;                   \
-    case 1 * 16 + 1: RUN(1, 1, 4, false); break;         \
-    case 1 * 16 + 2: RUN(2, 1, 4, false); break;         \
-    case 1 * 16 + 4: RUN(4, 1, 4, false); break;         \
-    case 4 * 16 + 1: RUN(1, 4, 4, false); break;         \
-    case 4 * 16 + 2: RUN(2, 4, 4, false); break;         \
-    case 4 * 16 + 4: RUN(4, 4, 4, false); break;         \
-    case 16 * 16 + 1: RUN(1, 16, 16, false); break;      \
-    case 16 * 16 + 2: RUN(2, 16, 16, false); break;      \
-    case 16 * 16 + 4: RUN(4, 16, 16, false); break;      \
-    default: RUN(8, 16, 16, false); break;               \
-  }
+int rn_rows_per_group(int lpr) { return lpr > 64 ? 1 : 256 / lpr; }
 
 template <class T, int MODE>
 int rn_launch_fwd(const RnFwd<T>& a, hipStream_t st) {
-  const RnShape sh = rn_shape(a.D, Elem<T>::VEC);
-  const unsigned grid = rn_grid(a.R, sh.wpr <= 1 ? 4 : 1, 8192);
-#define RN_F(NV, WPR, WAVES, SMALL) \
-  hipLaunchKernelGGL((k_rmsnorm_fwd<T, MODE, NV, WPR, WAVES, SMALL>), dim3(grid), dim3(64 * WAVES), 0, st, a)
-  RN_PICK(RN_F)
+  const RnShape sh = rn_shape(a.D, Elem<T>::VEC, MODE == RN_QUANT);
+  const dim3 grid(rn_grid(a.R, rn_rows_per_group(sh.lpr), 8192)), block(sh.lpr > 64 ? sh.lpr : 256);
+#define RN_F(LPR, NV, SMALL) hipLaunchKernelGGL((k_rmsnorm_fwd<T, MODE, NV, LPR, SMALL>), grid, block, 0, st, a)
+  constexpr bool Q = MODE == RN_QUANT;
+  switch (sh.lpr * 16 + sh.nv) {
+    case 8 * 16: RN_F(8, 1, true); break;
+    case 8 * 16 + 1: RN_F(8, 1, false); break;
+    case 16 * 16 + 1: RN_F(16, 1, false); break;
+    case 32 * 16 + 1: RN_F(32, 1, false); break;
+    case 64 * 16 + 1: RN_F(64, 1, false); break;
+    case 64 * 16 + 2: RN_F(64, 2, false); break;
+    case 64 * 16 + 4: if constexpr (Q) RN_F(64, 4, false); break;
+    case 256 * 16 + 1: if constexpr (!Q) RN_F(256, 1, false); break;
+    case 256 * 16 + 2: if constexpr (Q) RN_F(256, 2, false); break;
+    case 256 * 16 + 4: if constexpr (Q) RN_F(256, 4, false); break;
+    case 512 * 16 + 1: if constexpr (!Q) RN_F(512, 1, false); break;
+    case 512 * 16 + 2: if constexpr (!Q) RN_F(512, 2, false); break;
+    case 1024 * 16 + 2: RN_F(1024, 2, false); break;
+    case 1024 * 16 + 4: RN_F(1024, 4, false); break;
+    default: if constexpr (Elem<T>::VEC == 4) RN_F(1024, 8, false);
+  }
 #undef RN_F
   return hotk_launch_status();
 }
 
-unsigned rn_bwd_grid(int64_t R, int wpr) { return rn_grid(R, wpr <= 1 ? 4 : 1, 1024); }
+// workgroups of the backward pass, each with one partial row of dw: enough to fill the chip, few enough that the partial sums
+// stay a few percent of the traffic
+unsigned rn_bwd_grid(int64_t R, int lpr) { return rn_grid(R, rn_rows_per_group(lpr), lpr > 256 ? 512 : 1024); }
 
 template <class T>
 int rn_launch_bwd(const RnBwd<T>& a, hipStream_t st) {
-  const RnShape sh = rn_shape(a.D, Elem<T>::VEC);
-  const unsigned grid = rn_bwd_grid(a.R, sh.wpr);
-#define RN_B(NV, WPR, WAVES, SMALL) \
-  hipLaunchKernelGGL((k_rmsnorm_bwd<T, NV, WPR, WAVES, SMALL>), dim3(grid), dim3(64 * WAVES), 0, st, a)
-  RN_PICK(RN_B)
+  const RnShape sh = rn_shape(a.D, Elem<T>::VEC, false);
+  const dim3 grid(rn_bwd_grid(a.R, sh.lpr)), block(sh.lpr > 64 ? sh.lpr : 256);
+#define RN_B(LPR, NV, SMALL) hipLaunchKernelGGL((k_rmsnorm_bwd<T, NV, LPR, SMALL>), grid, block, 0, st, a)
+  switch (sh.lpr * 16 + sh.nv) {
+    case 8 * 16: RN_B(8, 1, true); break;
+    case 8 * 16 + 1: RN_B(8, 1, false); break;
+    case 16 * 16 + 1: RN_B(16, 1, false); break;
+    case 32 * 16 + 1: RN_B(32, 1, false); break;
+    case 64 * 16 + 1: RN_B(64, 1, false); break;
+    case 64 * 16 + 2: RN_B(64, 2, false); break;
+    case 256 * 16 + 1: RN_B(256, 1, false); break;
+    case 512 * 16 + 1: RN_B(512, 1, false); break;
+    case 512 * 16 + 2: RN_B(512, 2, false); break;
+    case 1024 * 16 + 2: RN_B(1024, 2, false); break;
+    case 1024 * 16 + 4: RN_B(1024, 4, false); break;
+    default: if constexpr (Elem<T>::VEC == 4) RN_B(1024, 8, false);
+  }
 #undef RN_B
   return hotk_launch_status();
 }
@@ -414,7 +433,7 @@ extern "C" int hotk_quantize_rows(const void* x, int64_t ld_x, uint8_t* q, float
 extern "C" int hotk_rmsnorm_partials(int64_t R, int64_t D, int type, int64_t* n_partials) {
   HOTK_CHECK_ARG(n_partials && R >= 0);
   if (!hotk_rmsnorm_supported(D, type)) return HOTK_EUNSUPPORTED;
-  *n_partials = (int64_t)rn_bwd_grid(R, rn_shape(D, 16 / ffn_bytes(type)).wpr);
+  *n_partials = (int64_t)rn_bwd_grid(R, rn_shape(D, 16 / ffn_bytes(type), false).lpr);
   return HOTK_OK;
 }
 
