@@ -368,16 +368,22 @@ void check_linear(const Tensor& x, const Tensor& w, const optional<Tensor>& b, c
   if (r) check_with(x, *r, "residual", result_shape(x, N), type);
 }
 
+// what the backward pass reads: the slopes, and the operands as rows (copies where the product made some)
+struct Kept {
+  Tensor save;
+  Rows x, w;
+};
 Tensor linear_forward(const Tensor& x, const Tensor& weight, const optional<Tensor>& b, const optional<Tensor>& r, int act, bool grad,
-                      Tensor* save) {
+                      Kept* kept) {
   const c10::DeviceGuard guard(x.device());
   const int64_t K = x.size(-1), N = weight.size(0);
   const Rows xs = padded(rows(x), K), ws = padded(rows(weight), K);
+  if (kept) *kept = {Tensor(), xs, ws};
   Extras e;
   e.act = act;
   if (b) e.bias = b->contiguous();
   e.res = rows(r);
-  if (grad && act) *save = e.save = like(x, {xs.n, N}, x.scalar_type() == at::kFloat ? at::kFloat : at::kShort);
+  if (grad && act) kept->save = e.save = like(x, {xs.n, N}, x.scalar_type() == at::kFloat ? at::kFloat : at::kShort);
   return product(xs, ws, xs.n, N, K, x.scalar_type(), e).view(result_shape(x, N));
 }
 
@@ -385,11 +391,15 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const optional<Tensor>& b, const optional<Tensor>& r,
                         int64_t act) {
     ctx->set_materialize_grads(false);
-    Tensor save;
+    Kept kept;
     const bool inner = wants_grad(x) || wants_grad(weight) || wants_grad(b);
-    const Tensor y = linear_forward(x, weight, b, r, (int)act, inner, &save);
-    ctx->save_for_backward({x, weight, save});
+    const Tensor y = linear_forward(x, weight, b, r, (int)act, inner, &kept);
+    // the input itself where it was read in place (so that a later change of it is noticed), else the copy
+    const bool own_x = !kept.x.t.is_same(x) && kept.x.n, own_w = !kept.w.t.is_same(weight);
+    ctx->save_for_backward({own_x ? kept.x.t : x, own_w ? kept.w.t : weight, kept.save});
     ctx->saved_data["act"] = act;
+    ctx->saved_data["shape"] = std::vector<int64_t>(x.sizes().begin(), x.sizes().end());
+    ctx->saved_data["ld"] = std::vector<int64_t>{own_x ? kept.x.ld : 0, own_w ? kept.w.ld : 0};
     ctx->saved_data["wants"] = (int64_t)(wants_grad(x) | wants_grad(weight) << 1 | wants_grad(b) << 2 | wants_grad(r) << 3);
     return y;
   }
@@ -398,15 +408,18 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &save = saved[2], &dy = g[0];
     const int act = (int)ctx->saved_data["act"].toInt();
-    const int64_t wants = ctx->saved_data["wants"].toInt(), K = x.size(-1), N = weight.size(0);
+    const int64_t wants = ctx->saved_data["wants"].toInt();
+    const auto shape = ctx->saved_data["shape"].toIntVector(), ld = ctx->saved_data["ld"].toIntVector();
+    const int64_t K = shape.back(), N = weight.size(0);
+    int64_t M = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) M *= shape[i];
     Tensor dx, dw, db;
     if (dy.defined() && (wants & 7)) {
       const c10::DeviceGuard guard(x.device());
       const auto type = x.scalar_type();
-      const int64_t M = x.numel() / K;
       if (M == 0) {
-        if (wants & 1) dx = at::zeros_like(x);
-        if (wants & 2) dw = at::zeros_like(weight);
+        if (wants & 1) dx = at::zeros(shape, x.options());
+        if (wants & 2) dw = at::zeros({N, K}, x.options());
         if (wants & 4) db = at::zeros({N}, x.options());
       } else {
         const Rows gs = rows(dy);
@@ -438,11 +451,11 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         Extras e;
         if (wants & 1) {
           e.flags = HOTK_LINEAR_W_DOWN;
-          dx = product(dz, padded(rows(weight), K), M, K, N, type, e).view(x.sizes());
+          dx = product(dz, ld[1] ? Rows{weight, ld[1], N} : rows(weight), M, K, N, type, e).view(shape);
         }
         if (wants & 2) {
           e.flags = HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN;
-          dw = product(dz, padded(rows(x), K), N, K, M, type, e);
+          dw = product(dz, ld[0] ? Rows{x, ld[0], M} : rows(x), N, K, M, type, e);
         }
       }
     }
@@ -456,8 +469,7 @@ Tensor linear_act(const Tensor& x, const Tensor& weight, const optional<Tensor>&
   check_linear(x, weight, b, r, x.scalar_type());
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(b) || wants_grad(r)))
     return LinearAct::apply(x, weight, b, r, (int64_t)code);
-  Tensor none;
-  return linear_forward(x, weight, b, r, code, false, &none);
+  return linear_forward(x, weight, b, r, code, false, nullptr);
 }
 
 Tensor linear_act_quantized(const Tensor& xq, const Tensor& x_scale, const Tensor& wq, const Tensor& w_scale, const optional<Tensor>& b,
