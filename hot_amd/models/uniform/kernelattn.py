@@ -46,7 +46,9 @@ class KernelSelfAttn(nn.Module):
         k = self.feature_map(k_raw, is_query=False)
         v = ops.RowsMatmul.apply(x, self.fc_v.weight.t(), self.fc_v.bias)
         att = ops.KernelAttn.apply(q, k, v, plan, ord_q, 1, self.feat_dim, self.dim_v_head, None)
-        return ops.RowsMatmul.apply(self.dropout(att), self.fc_o.weight.t(), self.fc_o.bias)
+        # (not the module's in-place form: att is a view made inside an autograd function, which may not be written to)
+        att = nn.functional.dropout(att, self.dropout.p, self.dropout.training)
+        return ops.RowsMatmul.apply(att, self.fc_o.weight.t(), self.fc_o.bias)
 
     def _1_to_1(self, x):
         h_1 = self.fc_1(x)
