@@ -323,9 +323,9 @@ struct Extras {
   Rows res;
   int act = HOTK_ACT_NONE, flags = 0;
 };
-// [M, N] = epilogue(x w^T), rows in whole pieces
-Tensor product(const Rows& x, const Rows& w, int64_t M, int64_t N, int64_t K, at::ScalarType type, const Extras& e) {
-  const Tensor y = like(x.t, {M, N}, type);
+// epilogue(x w^T) [M, N] as a new tensor of this shape (no view: the caller may go on in place), rows in whole pieces
+Tensor product(const Rows& x, const Rows& w, int64_t M, int64_t N, int64_t K, at::IntArrayRef shape, at::ScalarType type, const Extras& e) {
+  const Tensor y = like(x.t, shape, type);
   if (M == 0) return y;
   const int ty = type_of(x.t.scalar_type());
   hotk_linear_args a{};
@@ -384,7 +384,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& weight, const optional<Tens
   if (b) e.bias = b->contiguous();
   e.res = rows(r);
   if (grad && act) kept->save = e.save = like(x, {xs.n, N}, x.scalar_type() == at::kFloat ? at::kFloat : at::kShort);
-  return product(xs, ws, xs.n, N, K, x.scalar_type(), e).view(result_shape(x, N));
+  return product(xs, ws, xs.n, N, K, result_shape(x, N), x.scalar_type(), e);
 }
 
 struct LinearAct : torch::autograd::Function<LinearAct> {
@@ -451,11 +451,11 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         Extras e;
         if (wants & 1) {
           e.flags = HOTK_LINEAR_W_DOWN;
-          dx = product(dz, ld[1] ? Rows{weight, ld[1], N} : rows(weight), M, K, N, type, e).view(shape);
+          dx = product(dz, ld[1] ? Rows{weight, ld[1], N} : rows(weight), M, K, N, shape, type, e);
         }
         if (wants & 2) {
           e.flags = HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN;
-          dw = product(dz, ld[0] ? Rows{x, ld[0], M} : rows(x), N, K, M, type, e);
+          dw = product(dz, ld[0] ? Rows{x, ld[0], M} : rows(x), N, K, M, {N, K}, type, e);
         }
       }
     }
@@ -491,7 +491,7 @@ Tensor linear_act_quantized(const Tensor& xq, const Tensor& x_scale, const Tenso
   e.res = rows(r);
   e.x_scale = x_scale.contiguous();
   e.w_scale = w_scale.contiguous();
-  return product(padded(rows(xq), K), padded(rows(wq), K), xq.numel() / K, wq.size(0), K, type, e).view(result_shape(xq, wq.size(0)));
+  return product(padded(rows(xq), K), padded(rows(wq), K), xq.numel() / K, wq.size(0), K, result_shape(xq, wq.size(0)), type, e);
 }
 
 }  // namespace

@@ -8,13 +8,18 @@ nothing else.  This module holds the pieces the three stacks share, written once
   * `orders_and_widths`, the (order, width) schedule of a stack from its constructor arguments;
   * `pre_norm_block`, the LayerNorm -> Linear -> GELU -> Linear -> Dropout feed-forward block whose parameterised members
     sit at Sequential positions 0, 1 and 3 (keys `ffn.0.*`, `ffn.1.*`, `ffn.3.*`);
+  * `norm_of`, the norm that a stack's norm='layernorm' | 'rmsnorm' names, and `feed_forward`, the block over plain rows with
+    RMSNorm: norm, product with GELU, product with the residual, each one kernel;
   * `shared_feature_map`, the one FAVOR+ map an encoder hands to all its kernel-attention layers, and `maybe_redraw`.
 """
 from collections import namedtuple
 
+import torch
 import torch.nn as nn
 
+from .. import ops
 from .common.kernel import KernelFeatureMap
+from .common.rmsnorm import RMSNorm
 
 Layout = namedtuple('Layout', 'name linear apply nonlinear add kernel_attn readout_attn batch_type')
 
@@ -54,6 +59,34 @@ def orders_and_widths(ord_in, ord_hidden, ord_out, dim_in, dim_hidden, dim_out):
 def pre_norm_block(norm, first, act, second, drop):
     """feed-forward block; parameterised members at positions 0, 1, 3"""
     return nn.Sequential(norm, first, act, second, drop)
+
+
+def norm_of(name, dim):
+    if name not in ('layernorm', 'rmsnorm'):
+        raise AssertionError(f'unknown norm {name!r}')
+    return nn.LayerNorm(dim) if name == 'layernorm' else RMSNorm(dim)
+
+
+def feed_forward(ffn, x, residual=None, eight=None):
+    """h + ffn(h) for a pre_norm_block over rows with RMSNorm, nn.Linear and GELU, h = x (+ residual).  eight: the block's two
+    weights and their scales in 8 bits (quantize_block): the products then take 8-bit rows (no gradient)"""
+    norm, first, _, second, drop = ffn
+    if eight is not None:
+        w1, s1, w2, s2 = eight
+        q, s, *h = ops.rms_norm_quantized(x, norm.weight, residual, eps=norm.eps)
+        u = ops.linear_act_quantized(q, s, w1, s1, first.bias, act='gelu', out_dtype=x.dtype)
+        return ops.linear_act_quantized(*ops.quantize_rows(u), w2, s2, second.bias, residual=h[0] if h else x, out_dtype=x.dtype)
+    y, h = (norm(x), x) if residual is None else norm(x, residual)
+    u = ops.linear_act(y, first.weight, first.bias, act='gelu')
+    if drop.training and drop.p > 0:
+        return h + drop(ops.linear_act(u, second.weight, second.bias))
+    return ops.linear_act(u, second.weight, second.bias, residual=h)
+
+
+def quantize_block(ffn):
+    """a block's weights for feed_forward(eight=...): 8 bits with one scale per output column"""
+    with torch.no_grad():
+        return (*ops.quantize_rows(ffn[1].weight), *ops.quantize_rows(ffn[3].weight))
 
 
 def shared_feature_map(att_cfg, dim_qk, n_heads):

@@ -5,7 +5,8 @@ hot_pytorch/models/encoder.py:20-96; the assembly is table-driven (models/_stack
 (att_cfg 'kernel' / 'generalized_kernel') for output orders >= 1 and, as in the reference (encoder.py:34-35), the softmax
 readout SelfAttn(., 0) for an order-0 output, which is linear in |E|.  Quadratic softmax attention for output orders >= 1
 (att_cfg='default') is outside the linear-cost path: NotImplementedError.  The dense layout has the same readout
-(models/dense/attn.py)."""
+(models/dense/attn.py).  norm='rmsnorm' (not in the reference; the default is its LayerNorm) takes root-mean-square norms
+instead, with the padding mask in the same kernel."""
 import torch.nn as nn
 
 from . import _stack
@@ -16,7 +17,7 @@ class EncLayer(nn.Module):
     (`residual` False, as shipped)"""
 
     def __init__(self, ord_in, ord_out, dim_in, dim_qk, dim_v, dim_ff, n_heads, cfg='default', att_cfg='default',
-                 dropout=0., drop_mu=0., feature_map=None, sparse=True):
+                 dropout=0., drop_mu=0., feature_map=None, sparse=True, norm='layernorm'):
         super().__init__()
         if cfg not in ('default', 'local') or att_cfg not in ('default', 'kernel', 'generalized_kernel'):
             raise AssertionError(f'unknown configuration cfg={cfg!r}, att_cfg={att_cfg!r}')
@@ -24,11 +25,11 @@ class EncLayer(nn.Module):
         self.sparse = sparse
         self.residual = False
         self.add = lay.add()
-        self.ln = lay.apply(nn.LayerNorm(dim_in))
+        self.ln = lay.apply(_stack.norm_of(norm, dim_in))
         self.attn = self._attention(lay, ord_in, ord_out, dim_in, dim_qk, dim_v, n_heads, cfg, att_cfg, dropout, drop_mu,
                                     feature_map)
         self.ffn = _stack.pre_norm_block(
-            lay.apply(nn.LayerNorm(dim_in)),
+            lay.apply(_stack.norm_of(norm, dim_in)),
             lay.linear(ord_out, ord_out, dim_in, dim_ff, cfg='light'),
             lay.apply(nn.GELU(), skip_masking=True),
             lay.linear(ord_out, ord_out, dim_ff, dim_in, cfg='light'),
@@ -60,7 +61,7 @@ class Encoder(nn.Module):
 
     def __init__(self, ord_in, ord_out, ord_hidden: list, dim_in, dim_out, dim_hidden, dim_qk, dim_v, dim_ff, n_heads,
                  readout_dim_qk, readout_dim_v, readout_n_heads, enc_cfg='default', att_cfg='default',
-                 drop_input=0., dropout=0., drop_mu=0., sparse=True):
+                 drop_input=0., dropout=0., drop_mu=0., sparse=True, norm='layernorm'):
         super().__init__()
         lay = _stack.layout_of(sparse)
         self.sparse = sparse
@@ -74,9 +75,9 @@ class Encoder(nn.Module):
             # an order-0 layer is the readout and has its own attention widths
             qk, v, heads = (readout_dim_qk, readout_dim_v, readout_n_heads) if dst == 0 else (dim_qk, dim_v, n_heads)
             body.append(EncLayer(src, dst, dim_hidden, qk, v, dim_ff, heads, enc_cfg, att_cfg, dropout, drop_mu,
-                                 self.feature_map, sparse))
+                                 self.feature_map, sparse, norm))
         self.layers = nn.Sequential(*body)
-        self.output = lay.apply(nn.Sequential(nn.LayerNorm(dim_hidden), nn.Linear(dim_hidden, dim_out)))
+        self.output = lay.apply(nn.Sequential(_stack.norm_of(norm, dim_hidden), nn.Linear(dim_hidden, dim_out)))
 
     def forward(self, G):
         if not isinstance(G, self._batch_type):

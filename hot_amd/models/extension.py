@@ -2,14 +2,22 @@
 
 Interface contract of hot_pytorch/models/extension.py:14-124 (class names, constructor arguments, attribute names ->
 state_dict keys, forward(x, indices)); layers from hot_amd.models.uniform (HIP kernels), assembly shared with the other
-stacks (models/_stack.py).  Tensors are plain [N, D] / [B, D] here, so the pointwise members are torch modules."""
+stacks (models/_stack.py).  Tensors are plain [N, D] / [B, D] here, so the pointwise members are torch modules.
+
+norm='rmsnorm' (not in the reference; the default is its LayerNorm) takes root-mean-square norms, and the feed-forward block
+runs as three kernels: norm with the residual's addition, product with GELU, product with the block's skip.  Such an encoder
+can serve with 8-bit feed-forward products: Encoder.quantize_feed_forward()."""
 import torch
 import torch.nn as nn
 
+from .._lib import HotkError
 from . import _stack
 from .uniform.kernelattn import KernelSelfAttn
 from .uniform.f import Nonlinear, Add
 from .uniform.linear import Linear
+
+
+_EIGHT = ('ffn_w1_8bit', 'ffn_s1_8bit', 'ffn_w2_8bit', 'ffn_s2_8bit')     # buffers of a quantized block
 
 
 def _check_indices(indices):
@@ -27,7 +35,7 @@ def _only(value, allowed, what):
 
 class EncLayer(nn.Module):
     def __init__(self, ord_in, ord_out, dim_in, dim_qk, dim_v, dim_ff, n_heads, cfg='default', att_cfg='default',
-                 dropout=0., drop_mu=0., feature_map=None, sparse=False):
+                 dropout=0., drop_mu=0., feature_map=None, sparse=False, norm='layernorm'):
         super().__init__()
         _only(cfg, 'default', 'cfg')
         _only(att_cfg, 'generalized_kernel', 'att_cfg')
@@ -35,14 +43,34 @@ class EncLayer(nn.Module):
         self.ord_out = ord_out
         self.residual = False
         self.add = Add()
-        self.ln = nn.LayerNorm(dim_in)
+        self.norm = norm
+        self.ln = _stack.norm_of(norm, dim_in)
         # (dim_qk, dim_v) go positionally into the attention's (dim_v, dim_qk) parameters, as in extension.py:29
         self.attn = KernelSelfAttn(1, ord_out, dim_in, dim_qk, dim_v, n_heads, cfg, dropout, drop_mu, feature_map)
-        self.ffn = _stack.pre_norm_block(nn.LayerNorm(dim_in), nn.Linear(dim_in, dim_ff), nn.GELU(),
+        self.ffn = _stack.pre_norm_block(_stack.norm_of(norm, dim_in), nn.Linear(dim_in, dim_ff), nn.GELU(),
                                          nn.Linear(dim_ff, dim_in), nn.Dropout(dropout, inplace=True))
+
+    def quantize_feed_forward(self):
+        """keep the feed-forward weights in 8 bits too, for calls in eval mode without gradients; taken from the weights as they
+        are now: a forward call that finds them changed since raises.  They are not part of the state_dict"""
+        if self.norm != 'rmsnorm':
+            raise HotkError("8-bit feed-forward products need norm='rmsnorm'")
+        for name, t in zip(_EIGHT, _stack.quantize_block(self.ffn)):
+            self.register_buffer(name, t, persistent=False)
+        self._eight_of = self._versions()
+
+    def _versions(self):
+        return [self.ffn[i].weight._version for i in (1, 3)]
 
     def forward(self, x, indices=None):
         attended = self.attn(self.ln(x), indices)
+        if self.norm == 'rmsnorm':
+            eight = None
+            if not self.training and not torch.is_grad_enabled() and hasattr(self, _EIGHT[0]):
+                if self._eight_of != self._versions():
+                    raise HotkError('the feed-forward weights have changed since quantize_feed_forward(): call it again')
+                eight = [getattr(self, name) for name in _EIGHT]
+            return _stack.feed_forward(self.ffn, attended, x if self.residual else None, eight)
         if self.residual:
             attended = self.add(x, attended)
         return self.add(attended, self.ffn(attended))
@@ -51,7 +79,7 @@ class EncLayer(nn.Module):
 class Encoder(nn.Module):
     def __init__(self, ord_in, ord_out, ord_hidden: list, dim_in, dim_out, dim_hidden, dim_qk, dim_v, dim_ff, n_heads,
                  readout_dim_qk, readout_dim_v, readout_n_heads, enc_cfg='default', att_cfg='generalized_kernel',
-                 drop_input=0., dropout=0., drop_mu=0., sparse=False):
+                 drop_input=0., dropout=0., drop_mu=0., sparse=False, norm='layernorm'):
         super().__init__()
         _only(enc_cfg, 'default', 'enc_cfg')
         _only(att_cfg, 'generalized_kernel', 'att_cfg')
@@ -62,8 +90,14 @@ class Encoder(nn.Module):
         assert all(o == 1 for o in orders[:-1]), 'every layer input of this extension is a set (order 1)'
         self.layers = nn.ModuleList(
             EncLayer(1, dst, dim_hidden, dim_qk, dim_v, dim_ff, n_heads, enc_cfg, att_cfg, dropout, drop_mu,
-                     self.feature_map, sparse) for dst in orders[1:])
-        self.output = nn.Sequential(nn.LayerNorm(dim_hidden), nn.Linear(dim_hidden, dim_out))
+                     self.feature_map, sparse, norm) for dst in orders[1:])
+        self.output = nn.Sequential(_stack.norm_of(norm, dim_hidden), nn.Linear(dim_hidden, dim_out))
+
+    def quantize_feed_forward(self):
+        """8-bit feed-forward products in eval mode without gradients (EncLayer.quantize_feed_forward); returns self"""
+        for layer in self.layers:
+            layer.quantize_feed_forward()
+        return self
 
     def forward(self, x, indices):
         _check_indices(indices)

@@ -7,6 +7,7 @@ import torch.nn.functional as F
 
 from ...batch.sparse import Batch as B, apply, add_batch, batch_like
 from ... import ops
+from ..common.rmsnorm import RMSNorm
 
 
 class Apply(nn.Module):
@@ -23,6 +24,11 @@ class Apply(nn.Module):
                 kind = G.plan.kind if G.order == 2 else G.plan.nkind
             y = ops.LayerNormRows.apply(G.values, self.f.weight, self.f.bias, kind, self.f.eps)
             return batch_like(G, y, skip_masking=True)
+        if isinstance(self.f, RMSNorm) and isinstance(G, B):
+            kind = None
+            if not self.skip_masking and G._padded:
+                kind = G.plan.kind if G.order == 2 else G.plan.nkind
+            return batch_like(G, self.f(G.values, kind=kind), skip_masking=True)
         return apply(G, self.f, self.skip_masking)
 
 
