@@ -134,7 +134,7 @@ _SIGNATURES.update({
     'hotk_linear_workspace_bytes': [ctypes.POINTER(LinearArgs), ctypes.POINTER(_S)],
     'hotk_linear_act': [ctypes.POINTER(LinearArgs), _P, _S, _P],
     'hotk_linear_dz_partials': [_L, ctypes.POINTER(_L)],
-    'hotk_linear_dz': [_P, _L, _P, _I, _P, _L, _P, _L, _L, _I, _P],
+    'hotk_linear_dz': [_P, _L, _P, _I, _P, _L, _P, _P, _L, _L, _I, _P],
     'hotk_pad_rows': [_P, _L, _P, _L, _L, _L, _P],
 })
 EXPORTS = sorted(list(_SIGNATURES) + ['hotk_strerror', 'hotk_version'])

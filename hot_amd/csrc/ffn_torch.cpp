@@ -139,6 +139,7 @@ void check_with(const Tensor& ref, const Tensor& t, const char* what, at::IntArr
 struct Rows {
   Tensor t;
   int64_t ld = 0, n = 0;
+  bool zeros = false;                      // made here with zeros from a row's end to the next
   const void* p() const { return t.defined() ? t.const_data_ptr() : nullptr; }
 };
 
@@ -306,16 +307,16 @@ int64_t up(int64_t n, int64_t size) {      // n elements of `size` bytes in whol
   const int64_t m = 16 / size;
   return (n + m - 1) / m * m;
 }
-bool whole(const Rows& x, int64_t C) {     // rows as the product reads them: whole, aligned 16-byte pieces
+bool whole(const Rows& x, int64_t C) {     // rows as the tiles read them: whole, aligned 16-byte pieces, zeros behind the row
   const int64_t e = x.t.element_size();
-  return C * e % 16 == 0 && x.ld * e % 16 == 0 && (uintptr_t)x.p() % 16 == 0;
+  return (C * e % 16 == 0 || x.zeros) && x.ld * e % 16 == 0 && (uintptr_t)x.p() % 16 == 0;
 }
 Rows padded(const Rows& in, int64_t C) {   // itself where it is whole, else a copy with zeros behind each row
   if (in.n == 0 || whole(in, C)) return in;
   const int64_t e = in.t.element_size(), ld = up(C, e);
   const Tensor o = like(in.t, {in.n, ld}, in.t.scalar_type());
   launch("hotk_pad_rows", 2 * in.n * C * e, [&] { return L.pad_rows(in.p(), in.ld * e, o.data_ptr(), ld * e, in.n, C * e, stream_of(in.t)); });
-  return {o, ld, in.n};
+  return {o, ld, in.n, true};
 }
 
 struct Extras {
@@ -323,8 +324,10 @@ struct Extras {
   Rows res;
   int act = HOTK_ACT_NONE, flags = 0;
 };
-// epilogue(x w^T) [M, N] as a new tensor of this shape (no view: the caller may go on in place), rows in whole pieces
-Tensor product(const Rows& x, const Rows& w, int64_t M, int64_t N, int64_t K, at::IntArrayRef shape, at::ScalarType type, const Extras& e) {
+// epilogue(x w^T) [M, N] as a new tensor of this shape (no view: the caller may go on in place), copies of operands
+// that it had to make in `made`
+Tensor product(const Rows& x, const Rows& w, int64_t M, int64_t N, int64_t K, at::IntArrayRef shape, at::ScalarType type, const Extras& e,
+               Rows* made = nullptr) {
   const Tensor y = like(x.t, shape, type);
   if (M == 0) return y;
   const int ty = type_of(x.t.scalar_type());
@@ -338,8 +341,23 @@ Tensor product(const Rows& x, const Rows& w, int64_t M, int64_t N, int64_t K, at
   a.save = out(e.save);
   a.x_scale = (const float*)out(e.x_scale); a.w_scale = (const float*)out(e.w_scale);
   a.type = ty; a.out_type = type_of(type); a.act = e.act; a.flags = e.flags;
+  if (x.zeros && (w.zeros || (a.flags & HOTK_LINEAR_W_DOWN))) a.flags |= HOTK_LINEAR_PADDED;
   size_t need = 0;
-  check(L.linear_workspace_bytes(&a, &need), "hotk_linear_act");
+  int rc = L.linear_workspace_bytes(&a, &need);
+  Rows copies[2];
+  if (rc == HOTK_EUNSUPPORTED && !(a.flags & HOTK_LINEAR_X_DOWN)) {      // not in whole pieces: copies that are
+    copies[0] = padded(x, K);
+    copies[1] = padded(w, a.flags & HOTK_LINEAR_W_DOWN ? N : K);
+    a.x = copies[0].p(); a.ld_x = copies[0].ld;
+    a.w = copies[1].p(); a.ld_w = copies[1].ld;
+    a.flags |= HOTK_LINEAR_PADDED;       // (a row that needed no copy ends with a piece)
+    rc = L.linear_workspace_bytes(&a, &need);
+    if (made) {
+      made[0] = copies[0];
+      made[1] = copies[1];
+    }
+  }
+  check(rc, "hotk_linear_act");
   const Tensor ws = need ? like(x.t, {(int64_t)need}, at::kByte) : Tensor();
   launch("hotk_linear_act", (M + N) * K * x.t.element_size() + M * N * y.element_size() * (1 + e.res.t.defined()),
          [&] { return L.linear_act(&a, out(ws), need, stream_of(x.t)); });
@@ -377,14 +395,19 @@ Tensor linear_forward(const Tensor& x, const Tensor& weight, const optional<Tens
                       Kept* kept) {
   const c10::DeviceGuard guard(x.device());
   const int64_t K = x.size(-1), N = weight.size(0);
-  const Rows xs = padded(rows(x), K), ws = padded(rows(weight), K);
-  if (kept) *kept = {Tensor(), xs, ws};
+  const Rows xs = rows(x), ws = rows(weight);
   Extras e;
   e.act = act;
   if (b) e.bias = b->contiguous();
   e.res = rows(r);
   if (grad && act) kept->save = e.save = like(x, {xs.n, N}, x.scalar_type() == at::kFloat ? at::kFloat : at::kShort);
-  return product(xs, ws, xs.n, N, K, result_shape(x, N), x.scalar_type(), e);
+  Rows made[2] = {xs, ws};
+  const Tensor y = product(xs, ws, xs.n, N, K, result_shape(x, N), x.scalar_type(), e, made);
+  if (kept) {
+    kept->x = made[0];
+    kept->w = made[1];
+  }
+  return y;
 }
 
 struct LinearAct : torch::autograd::Function<LinearAct> {
@@ -429,33 +452,33 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         const bool itself = act == HOTK_ACT_NONE && whole(gs, N);
         if ((wants & 3) && !itself) {
           const int64_t ld = up(N, x.element_size());
-          dz = {like(x, {M, ld}, type), ld, M};
+          dz = {like(x, {M, ld}, type), ld, M, true};
         }
         Tensor part;
         if (wants & 4) {
           int64_t n = 0;
           check(L.linear_dz_partials(M, &n), "hotk_linear_dz_partials");
-          part = like(x, {n, N}, at::kFloat);
+          db = like(x, {N}, type);
+          if (n > 1) part = like(x, {n, N}, at::kFloat);
         }
         const bool write = (wants & 3) && !itself;
-        if (write || part.defined())
+        if (write || db.defined())
           launch("hotk_linear_dz", M * N * x.element_size() * (1 + write + (act != HOTK_ACT_NONE)), [&] {
-            return L.linear_dz(gs.p(), gs.ld, out(save), act, write ? dz.t.data_ptr() : nullptr, dz.ld, (float*)out(part), M, N, ty, stream_of(x));
+            return L.linear_dz(gs.p(), gs.ld, out(save), act, write ? dz.t.data_ptr() : nullptr, dz.ld, (float*)out(part), part.defined() ? nullptr : out(db),
+                               M, N, ty, stream_of(x));
           });
-        if (wants & 4) {
-          db = like(x, {N}, type);
+        if (part.defined())
           launch("hotk_sum_partials", 4 * part.numel(), [&] {
             return L.sum_partials(part.const_data_ptr<float>(), part.size(0), N, db.data_ptr(), ty, stream_of(x));
           });
-        }
         Extras e;
         if (wants & 1) {
           e.flags = HOTK_LINEAR_W_DOWN;
-          dx = product(dz, ld[1] ? Rows{weight, ld[1], N} : rows(weight), M, K, N, shape, type, e);
+          dx = product(dz, padded(ld[1] ? Rows{weight, ld[1], N, true} : rows(weight), K), M, K, N, shape, type, e);
         }
         if (wants & 2) {
           e.flags = HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN;
-          dw = product(dz, ld[0] ? Rows{x, ld[0], M} : rows(x), N, K, M, {N, K}, type, e);
+          dw = product(dz, padded(ld[0] ? Rows{x, ld[0], M, true} : rows(x), K), N, K, M, {N, K}, type, e);
         }
       }
     }
@@ -491,7 +514,7 @@ Tensor linear_act_quantized(const Tensor& xq, const Tensor& x_scale, const Tenso
   e.res = rows(r);
   e.x_scale = x_scale.contiguous();
   e.w_scale = w_scale.contiguous();
-  return product(padded(rows(xq), K), padded(rows(wq), K), xq.numel() / K, wq.size(0), K, result_shape(xq, wq.size(0)), type, e);
+  return product(rows(xq), rows(wq), xq.numel() / K, wq.size(0), K, result_shape(xq, wq.size(0)), type, e);
 }
 
 }  // namespace

@@ -522,25 +522,42 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linact_tile(const LaTile<OT> g
   }
 }
 
-// joins the splits in order and finishes: eight columns a thread
+// joins the splits and finishes: a workgroup takes 32 pieces of V columns, eight threads a piece, each adding every eighth split
+// in order; the eight meet in LDS, again in order
 template <class OT>
 __global__ __launch_bounds__(256) void k_linact_join(const float* __restrict__ part, int splits, int64_t M, int64_t N,
                                                      const LaEpi<OT> e) {
-  const int64_t per_row = (N + 7) / 8, total = M * per_row;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
-    const int64_t m = t / per_row, n = t % per_row * 8;
-    const int left = (int)(N - n < 8 ? N - n : 8);
-    float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s) {
-      const float* row = part + ((int64_t)s * M + m) * N + n;
+  constexpr int V = Elem<OT>::VEC;
+  __shared__ __align__(16) float sums[8][32][V];
+  const int64_t per_row = (N + V - 1) / V, total = M * per_row;
+  const int piece = threadIdx.x & 31, lane = threadIdx.x >> 5;
+  for (int64_t t0 = (int64_t)blockIdx.x * 32; t0 < total; t0 += (int64_t)gridDim.x * 32) {
+    const int64_t t = t0 + piece, m = t / per_row, n = t % per_row * V;
+    const int left = (int)(N - n < V ? N - n : V);
+    float z[V];
 #pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        const f32x4 v = ffn_load(row, i, left);
+    for (int k = 0; k < V; ++k) z[k] = 0.f;
+    if (t < total)
+      for (int s = lane; s < splits; s += 8) {
+        const float* row = part + ((int64_t)s * M + m) * N + n;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) z[i + k] += v[k];
+        for (int i = 0; i < V; i += 4) {
+          const f32x4 v = ffn_load(row, i, left);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) z[i + k] += v[k];
+        }
       }
+#pragma unroll
+    for (int i = 0; i < V; i += 4) *reinterpret_cast<f32x4*>(&sums[lane][piece][i]) = f32x4{z[i], z[i + 1], z[i + 2], z[i + 3]};
+    __syncthreads();
+    if (lane == 0 && t < total) {
+      const int parts = splits < 8 ? splits : 8;
+      for (int s = 1; s < parts; ++s)
+#pragma unroll
+        for (int k = 0; k < V; ++k) z[k] += sums[s][piece][k];
+      la_finish<V>(e, m, n, N, z);
     }
-    la_finish<8>(e, m, n, N, z);
+    __syncthreads();
   }
 }
 
@@ -556,7 +573,7 @@ __global__ __launch_bounds__(512) void k_linact_few(const LaTile<OT> g) {
   constexpr int U = MB == 1 ? 4 : MB == 2 ? 2 : 1;                 // (registers: 8 U (1 + MB) of them hold pieces under way)
   __shared__ __align__(16) float sums[WAVES][MB * 16][PITCH];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * 16, chunks = (g.K * E + 15) / 16;
+  const int64_t n0 = (int64_t)blockIdx.x * 16, bytes = g.K * E;
   const char* wrow = g.b + (n0 + lr < g.N ? n0 + lr : g.N - 1) * g.ldb;
   const char* xrow[MB];
   f32x4 acc[MB];
@@ -565,9 +582,22 @@ __global__ __launch_bounds__(512) void k_linact_few(const LaTile<OT> g) {
     xrow[b] = g.a + (16 * b + lr < g.M ? 16 * b + lr : g.M - 1) * g.lda;
     acc[b] = 0.f;
   }
+  // rows may start anywhere and end inside a piece: what lies behind the end is not read, and counts as zero
   auto piece = [&](const char* row, int64_t c) {
+    typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(1)));
     u32x4 v = 0;
-    if (c < chunks) v = *reinterpret_cast<const u32x4*>(row + c * 16);
+    const int64_t at = c * 16;
+    if (at + 16 <= bytes) {
+      v = *reinterpret_cast<const u32x4u*>(row + at);
+    } else if (at < bytes) {
+#pragma unroll
+      for (int i = 0; i < 16; i += E)
+        if (at + i < bytes) {
+          if (E == 4) v[i / 4] = *reinterpret_cast<const uint32_t*>(row + at + i);
+          else if (E == 2) v[i / 4] |= (uint32_t)*reinterpret_cast<const uint16_t*>(row + at + i) << (8 * (i & 3));
+          else v[i / 4] |= (uint32_t)*reinterpret_cast<const uint8_t*>(row + at + i) << (8 * (i & 3));
+        }
+    }
     return v;
   };
   for (int k0 = wave; k0 < g.ktiles; k0 += WAVES * U) {
@@ -619,12 +649,13 @@ __global__ __launch_bounds__(512) void k_linact_few(const LaTile<OT> g) {
 }
 
 // ---- backward: dz and its column sums; rows padded to whole pieces ---------------------------------------------------------
-// v = in * slope over a block of `rows` rows: out [R, ld_out] with zeros from C on, partial [block][C] the block's column sums.
+// v = in * slope over a block of `rows` rows: out [R, ld_out] with zeros from C on, partial [block][C] the block's column sums, or
+// total [C] where there is one block.
 // A thread owns one 16-byte piece of columns and every (256 / cg)th row of the block; cg (a power of two) pieces go side by side
 template <class T>
 __global__ __launch_bounds__(256) void k_linact_dz(const T* __restrict__ in, int64_t ld_in, const void* __restrict__ save, int act,
-                                                   T* __restrict__ out, int64_t ld_out, float* __restrict__ partial, int64_t R,
-                                                   int64_t C, int rows, int cg_log, unsigned across) {
+                                                   T* __restrict__ out, int64_t ld_out, float* __restrict__ partial,
+                                                   T* __restrict__ total, int64_t R, int64_t C, int rows, int cg_log, unsigned across) {
   using E = Elem<T>;
   using FV = typename E::fvec;
   __shared__ FV sums[256];
@@ -661,14 +692,17 @@ __global__ __launch_bounds__(256) void k_linact_dz(const T* __restrict__ in, int
       if (out && room > 0) ffn_store(out + r * ld_out + c, 0, room, v);
     }
   }
-  if (partial) {
+  if (partial || total) {
     sums[threadIdx.x] = s;
     __syncthreads();
     if (rl == 0) {
       for (int i = 1; i < rstep; ++i) s += sums[(i << cg_log) + piece];
 #pragma unroll
       for (int k = 0; k < E::VEC; ++k)
-        if (k < left) partial[block * C + c + k] = s[k];
+        if (k < left) {
+          if (total) total[c + k] = (T)s[k];
+          else partial[block * C + c + k] = s[k];
+        }
     }
   }
 }
@@ -702,7 +736,7 @@ int64_t la_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct LaShape { int bm, bn, splits; };      // bn 16: k_linact_few, bm / 16 blocks of rows
 struct LaCost { int bm, bn; float sat, lat, end; };
 const LaCost LA_COSTS[] = {{256, 256, 1.58f, 1.58f, 6.f}, {128, 128, 0.42f, 0.69f, 3.f}, {64, 128, 0.26f, 0.39f, 1.2f}, {64, 64, 0.16f, 0.32f, 0.7f}};
-LaShape la_shape(int64_t M, int64_t N, int64_t K, int type, int out_type, int flags) {
+LaShape la_shape(int64_t M, int64_t N, int64_t K, int type, int out_type, int flags, bool whole) {
   const int64_t ktiles = la_div(K * ffn_bytes(type), 128);
   const bool wide = type == HOTK_E4M3 && out_type == HOTK_F32;
   const float mfma = type == HOTK_F32 ? 8.f : wide ? 2.f : 1.f;
@@ -711,7 +745,8 @@ LaShape la_shape(int64_t M, int64_t N, int64_t K, int type, int out_type, int fl
   if (M <= 64 && flags == 0) {               // k_linact_few: 8.6 TB/s in all, 50 GB/s a compute unit, its matrix work beside that
     const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
     const float wgs = (float)la_div(N, 16), bytes = ktiles * 128.f * 16 * (1 + mb);
-    least = std::max(std::max(wgs * bytes / 8.6e6f, std::ceil(wgs / 256.f) * bytes / 50e3f),
+    // (rows in no whole pieces: the tiles would need two copies first)
+    least = -(whole ? 0.f : 8.f) + std::max(std::max(wgs * bytes / 8.6e6f, std::ceil(wgs / 256.f) * bytes / 50e3f),
                      std::ceil(wgs / 256.f) * ktiles * 0.89f * mfma * mb / 256.f);
     best = {16 * mb, 16, 1};
   }
@@ -735,6 +770,8 @@ LaShape la_shape(int64_t M, int64_t N, int64_t K, int type, int out_type, int fl
   }
   return best;
 }
+
+LaShape la_shape(const hotk_linear_args& a);
 
 template <class IT, class OT, int MB>
 int la_run_few(const LaTile<OT>& g, hipStream_t st) {
@@ -767,7 +804,7 @@ template <class IT, class OT, bool TA, bool TB>
 int la_product(const hotk_linear_args& a, void* ws, size_t nws, hipStream_t st) {
   const int e = ffn_bytes(a.type);
   const int64_t ktiles = la_div(a.K * e, 128);
-  const LaShape s = la_shape(a.M, a.N, a.K, a.type, a.out_type, a.flags);
+  const LaShape s = la_shape(a);
   const size_t need = s.splits > 1 ? (size_t)s.splits * a.M * a.N * 4 : 0;
   if (nws < need || (need && !ws)) return HOTK_EWORKSPACE;
   LaTile<OT> g{};
@@ -784,30 +821,41 @@ int la_product(const hotk_linear_args& a, void* ws, size_t nws, hipStream_t st) 
          : s.bn == 128 ? la_run<IT, OT, TA, TB, 64, 128, 2, 2>(g, s.splits, st)
                        : la_run<IT, OT, TA, TB, 64, 64, 4, 1>(g, s.splits, st);
   if (rc == HOTK_OK && need) {
-    const int64_t work = a.M * la_div(a.N, 8);
-    hipLaunchKernelGGL(k_linact_join<OT>, dim3(hotk_grid(work, 256)), dim3(256), 0, st, (const float*)ws, s.splits, a.M, a.N, g.e);
+    const int64_t work = a.M * la_div(a.N, Elem<OT>::VEC);
+    hipLaunchKernelGGL(k_linact_join<OT>, dim3(hotk_grid(work, 32, 256 * 32)), dim3(256), 0, st, (const float*)ws, s.splits, a.M, a.N, g.e);
     rc = hotk_launch_status();
   }
   return rc;
 }
 
+// rows of x and w in whole, aligned 16-byte pieces, with zeros behind the contraction's end
+bool la_whole(const hotk_linear_args& a) {
+  const int e = ffn_bytes(a.type), m = 16 / e;
+  const int64_t row_x = a.flags & HOTK_LINEAR_X_DOWN ? a.M : a.K, row_w = a.flags & HOTK_LINEAR_W_DOWN ? a.N : a.K;
+  if (a.K % m && !(a.flags & (HOTK_LINEAR_PADDED | HOTK_LINEAR_X_DOWN))) return false;
+  return a.ld_x >= la_div(row_x, m) * m && a.ld_w >= la_div(row_w, m) * m && (a.ld_x * e) % 16 == 0 && (a.ld_w * e) % 16 == 0 &&
+         hotk_aligned16(a.x) && hotk_aligned16(a.w);
+}
+LaShape la_shape(const hotk_linear_args& a) { return la_shape(a.M, a.N, a.K, a.type, a.out_type, a.flags & (HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN), la_whole(a)); }
+
 int la_check(const hotk_linear_args& a) {
   HOTK_CHECK_ARG(a.M >= 0 && a.N > 0 && a.K > 0);
   if (!(ffn_type_ok(a.type) || a.type == HOTK_E4M3) || !ffn_type_ok(a.out_type)) return HOTK_EUNSUPPORTED;
   if (a.type != HOTK_E4M3 && a.out_type != a.type) return HOTK_EUNSUPPORTED;
-  HOTK_CHECK_ARG((a.flags & ~(HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN)) == 0);
-  if (a.flags == HOTK_LINEAR_X_DOWN || (a.flags && a.type == HOTK_E4M3)) return HOTK_EUNSUPPORTED;
+  HOTK_CHECK_ARG((a.flags & ~(HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN | HOTK_LINEAR_PADDED)) == 0);
+  const int down = a.flags & (HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN);
+  if (down == HOTK_LINEAR_X_DOWN || (down && a.type == HOTK_E4M3)) return HOTK_EUNSUPPORTED;
   HOTK_CHECK_ARG(a.act >= HOTK_ACT_NONE && a.act <= HOTK_ACT_SILU);
   HOTK_CHECK_ARG((a.type == HOTK_E4M3) == (a.x_scale != nullptr) && (a.x_scale != nullptr) == (a.w_scale != nullptr));
   HOTK_CHECK_ARG(a.type != HOTK_E4M3 || !a.save);
-  const int e = ffn_bytes(a.type), m = 16 / e;
-  // operands in rows of whole, aligned 16-byte pieces (the caller pads others: hotk_pad_rows)
+  const int e = ffn_bytes(a.type);
   const int64_t row_x = a.flags & HOTK_LINEAR_X_DOWN ? a.M : a.K, row_w = a.flags & HOTK_LINEAR_W_DOWN ? a.N : a.K;
   HOTK_CHECK_ARG(a.ld_x >= row_x && a.ld_w >= row_w && a.ld_y >= a.N && (!a.res || a.ld_res >= a.N));
-  if (a.ld_x < la_div(row_x, m) * m || a.ld_w < la_div(row_w, m) * m || (a.ld_x * e) % 16 || (a.ld_w * e) % 16) return HOTK_EUNSUPPORTED;
   if (a.M > 0) {
     HOTK_CHECK_ARG(a.x && a.w && a.y);
-    if (!hotk_aligned16(a.x) || !hotk_aligned16(a.w)) return HOTK_EUNSUPPORTED;
+    HOTK_CHECK_ARG(ffn_elem_aligned(a.x, a.type) && ffn_elem_aligned(a.w, a.type));
+    // the tiles read rows in whole, aligned 16-byte pieces (the caller pads others: hotk_pad_rows)
+    if (!la_whole(a) && la_shape(a).bn != 16) return HOTK_EUNSUPPORTED;
     HOTK_CHECK_ARG(ffn_elem_aligned(a.y, a.out_type) && ffn_elem_aligned(a.bias, a.out_type) && ffn_elem_aligned(a.res, a.out_type));
     HOTK_CHECK_ARG(((uintptr_t)a.save) % (a.out_type == HOTK_F32 ? 4 : 2) == 0);
     HOTK_CHECK_ARG(((uintptr_t)a.x_scale) % 4 == 0 && ((uintptr_t)a.w_scale) % 4 == 0);
@@ -818,15 +866,16 @@ int la_check(const hotk_linear_args& a) {
   return HOTK_OK;
 }
 
-// rows of a block of hotk_linear_dz: 16, and more where that would be over 512 blocks of column sums
-int64_t la_dz_rows(int64_t R) { return la_div(la_div(R, 512), 16) * 16; }
+// rows of a block of hotk_linear_dz: all of up to 64 (one block: its sums are the result), else 16, and more where that would be
+// over 512 blocks
+int64_t la_dz_rows(int64_t R) { return R <= 64 ? 64 : la_div(la_div(R, 512), 16) * 16; }
 
 }  // namespace
 
 extern "C" int hotk_linear_workspace_bytes(const hotk_linear_args* args, size_t* bytes) {
   HOTK_CHECK_ARG(args && bytes);
   if (const int rc = la_check(*args)) return rc;
-  const LaShape s = la_shape(args->M, args->N, args->K, args->type, args->out_type, args->flags);
+  const LaShape s = la_shape(*args);
   *bytes = s.splits > 1 ? (size_t)s.splits * args->M * args->N * 4 : 0;
   return HOTK_OK;
 }
@@ -842,8 +891,8 @@ extern "C" int hotk_linear_act(const hotk_linear_args* args, void* workspace, si
     using T8 = std::conditional_t<std::is_same<OT, float>::value, e4m3_wide, e4m3>;
       using T8 = std::conditional_t<std::is_same<OT, float>::value, e4m3_wide, e4m3>;
     rc = args->type == HOTK_E4M3 ? la_product<T8, OT, false, false>(*args, workspace, ws_bytes, st)
-       : args->flags == 0 ? la_product<OT, OT, false, false>(*args, workspace, ws_bytes, st)
-       : args->flags == HOTK_LINEAR_W_DOWN ? la_product<OT, OT, false, true>(*args, workspace, ws_bytes, st)
+       : !(args->flags & HOTK_LINEAR_W_DOWN) ? la_product<OT, OT, false, false>(*args, workspace, ws_bytes, st)
+       : !(args->flags & HOTK_LINEAR_X_DOWN) ? la_product<OT, OT, false, true>(*args, workspace, ws_bytes, st)
                                            : la_product<OT, OT, true, true>(*args, workspace, ws_bytes, st);
   });
   return rc;
@@ -856,11 +905,12 @@ extern "C" int hotk_linear_dz_partials(int64_t R, int64_t* n_partials) {
 }
 
 extern "C" int hotk_linear_dz(const void* in, int64_t ld_in, const void* save, int act, void* out, int64_t ld_out, float* partial,
-                              int64_t R, int64_t C, int type, void* stream) {
-  HOTK_CHECK_ARG(R >= 0 && C > 0 && ld_in >= C && (!out || ld_out >= C) && (out || partial));
+                              void* total, int64_t R, int64_t C, int type, void* stream) {
+  HOTK_CHECK_ARG(R >= 0 && C > 0 && ld_in >= C && (!out || ld_out >= C) && (out || partial || total));
+  HOTK_CHECK_ARG(!total || (!partial && R <= la_dz_rows(R)));
   HOTK_CHECK_ARG(act >= HOTK_ACT_NONE && act <= HOTK_ACT_SILU && (act == HOTK_ACT_NONE || save || R == 0));
   if (!ffn_type_ok(type)) return HOTK_EUNSUPPORTED;
-  HOTK_CHECK_ARG(ffn_elem_aligned(in, type) && ffn_elem_aligned(out, type) && ((uintptr_t)save) % (type == HOTK_F32 ? 4 : 2) == 0 &&
+  HOTK_CHECK_ARG(ffn_elem_aligned(in, type) && ffn_elem_aligned(out, type) && ffn_elem_aligned(total, type) && ((uintptr_t)save) % (type == HOTK_F32 ? 4 : 2) == 0 &&
                  ((uintptr_t)partial) % 4 == 0);
   if (R == 0) return HOTK_OK;
   HOTK_CHECK_ARG(in);
@@ -872,7 +922,7 @@ extern "C" int hotk_linear_dz(const void* in, int64_t ld_in, const void* save, i
   ffn_dispatch(type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     hipLaunchKernelGGL(k_linact_dz<T>, dim3((unsigned)(across * down)), dim3(256), 0, (hipStream_t)stream, (const T*)in, ld_in, save, act,
-                       (T*)out, ld_out, partial, R, C, (int)rows, cg_log, (unsigned)across);
+                       (T*)out, ld_out, partial, (T*)total, R, C, (int)rows, cg_log, (unsigned)across);
   });
   return hotk_launch_status();
 }

@@ -538,12 +538,13 @@ int hotk_sum_partials(const float* partial, int64_t n, int64_t D, void* out, int
  * w_scale[n] (x w^T) + bias, with bias, res and y in out_type; otherwise out_type = type.  save (NULL: none) [M, N]: what
  * hotk_linear_dz needs for the gradient, int16 for 16-bit types, fp32 for HOTK_F32; not written for HOTK_ACT_NONE.
  * flags: the contraction runs down the columns of w [K, N] (a gradient of x), or of both w and x [K, M] (a gradient of w).
- * Rows of x and w lie in whole, aligned 16-byte pieces (their strides and both pointers; else HOTK_EUNSUPPORTED: hotk_pad_rows
- * makes copies).  What lies between a row's end and its piece's end: zeros where the contraction runs along the rows, anything
- * where it runs down them. */
+ * Rows of x and w lie in whole, aligned 16-byte pieces (their strides and both pointers), or HOTK_EUNSUPPORTED, here and from
+ * hotk_linear_workspace_bytes: hotk_pad_rows makes copies.  (Few rows of x are taken at any alignment.)  HOTK_LINEAR_PADDED: a
+ * contraction that runs along rows and ends inside a piece has zeros up to the piece's end, in each operand it runs along;
+ * without it K has to be whole pieces there.  Where a contraction runs down, the rest of a row's last piece may hold anything. */
 enum { HOTK_ACT_NONE = 0, HOTK_ACT_RELU = 1, HOTK_ACT_LEAKYRELU = 2 /* slope 0.01 */, HOTK_ACT_GELU = 3 /* exact, by erf */,
        HOTK_ACT_TANH = 4, HOTK_ACT_SILU = 5 };
-enum { HOTK_LINEAR_X_DOWN = 1, HOTK_LINEAR_W_DOWN = 2 };
+enum { HOTK_LINEAR_X_DOWN = 1, HOTK_LINEAR_W_DOWN = 2, HOTK_LINEAR_PADDED = 4 };
 typedef struct {
   int64_t M, N, K;
   const void* x; int64_t ld_x;
@@ -559,10 +560,11 @@ typedef struct {
 int hotk_linear_workspace_bytes(const hotk_linear_args* args, size_t* bytes);       /* for exactly these arguments */
 int hotk_linear_act(const hotk_linear_args* args, void* workspace, size_t ws_bytes, void* stream);
 /* v = in [R, C] times the slope that `save` holds (HOTK_ACT_NONE: times one); out (NULL: none) [R, ld_out], with zeros from C on;
- * partial (NULL: none) [n][C], n = hotk_linear_dz_partials(R): column sums of v in 32 bits, for hotk_sum_partials */
+ * partial (NULL: none) [n][C], n = hotk_linear_dz_partials(R): column sums of v in 32 bits, for hotk_sum_partials; total (NULL:
+ * none) [C]: the sums themselves, rounded to the type, instead of partial where n is 1 */
 int hotk_linear_dz_partials(int64_t R, int64_t* n_partials);
-int hotk_linear_dz(const void* in, int64_t ld_in, const void* save, int act, void* out, int64_t ld_out, float* partial, int64_t R,
-                   int64_t C, int type, void* stream);
+int hotk_linear_dz(const void* in, int64_t ld_in, const void* save, int act, void* out, int64_t ld_out, float* partial,
+                   void* total, int64_t R, int64_t C, int type, void* stream);
 /* rows of `bytes` bytes, ld_in bytes apart, copied to rows ld_out bytes apart (a multiple of 16, out 16-byte aligned) with zeros
  * behind them */
 int hotk_pad_rows(const void* in, int64_t ld_in, void* out, int64_t ld_out, int64_t R, int64_t bytes, void* stream);

@@ -439,6 +439,36 @@ def eight_bit_sums(xq, xs, wq, ws, out):
     return 2.0 ** -10 * (xq.double().abs() * xs.double()[:, None]) @ (wq.double().abs() * ws.double()[:, None]).t()
 
 
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('M', [3, 40, 100, 700])
+@pytest.mark.parametrize('K', [1, 5, 101, 133])
+def test_product_reads_nothing_behind_a_row(M, K, dt):
+    """rows that end inside a 16-byte piece, with NaN behind and before them: at stride and start that look aligned, and at odd ones"""
+    from hot_amd import ops
+    N = 70
+    x, w, b, _ = linear_case(M, N, K, dt, True, False, seed=230)
+    want = ops.linear_act(x, w, b, act='relu')
+    z, dz = z_bounds(x, w, b)
+    check_forward(want, z, dz, 'relu', None, dt)
+    dy = rnd(231, M, N + 1, dt=dt)
+    ref = torch.autograd.grad(ops.linear_act(x.requires_grad_(True), w.requires_grad_(True), b, act='relu'), (x, w), dy[:, :N].contiguous())
+    for start, width in ((16, 16 + 160), (3, 16 + 161)):
+        bx, bw = (torch.full((n, width), float('nan'), dtype=dt, device=DEV) for n in (M, N))
+        xv, wv = bx[:, start:start + K], bw[:, start:start + K]
+        xv.copy_(x.detach()), wv.copy_(w.detach())
+        assert torch.equal(ops.linear_act(xv, wv, b, act='relu'), want)
+        xv, wv = xv.detach().requires_grad_(True), wv.detach().requires_grad_(True)
+        got = torch.autograd.grad(ops.linear_act(xv, wv, b, act='relu'), (xv, wv), dy[:, :N])
+        assert all(torch.equal(g, r) for g, r in zip(got, ref))
+    if dt == torch.bfloat16 and K > 1:
+        q, s = ops.quantize_rows(x.detach())
+        wq, ws = ops.quantize_rows(w.detach())
+        want = ops.linear_act_quantized(q, s, wq, ws, b)
+        bq = torch.full((M, 208), float('nan'), device=DEV).to(E4M3)
+        bq[:, 16:16 + K] = q
+        assert torch.equal(ops.linear_act_quantized(bq[:, 16:16 + K], s, wq, ws, b), want)
+
+
 @pytest.mark.parametrize('out', TYPES)
 @pytest.mark.parametrize('M,N,K', [(1, 1, 1), (1, 33, 16), (5, 64, 48), (16, 100, 4096), (17, 65, 130), (33, 16, 272), (130, 257, 1000), (700, 520, 144),
                                    (3000, 1100, 80), (2, 2050, 512)])
