@@ -522,42 +522,44 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linact_tile(const LaTile<OT> g
   }
 }
 
-// joins the splits and finishes: a workgroup takes 32 pieces of V columns, eight threads a piece, each adding every eighth split
-// in order; the eight meet in LDS, again in order
-template <class OT>
+// joins the splits and finishes: LANES threads a piece of V columns, each adding every LANES-th split in order; they meet in LDS,
+// again in order.  One thread a piece for up to four splits, eight for more (4 096 x 1 024 of two splits: 8.6 us against 17;
+// 256 x 256 fp32 of sixteen: 6.7 against 3.9)
+template <class OT, int LANES>
 __global__ __launch_bounds__(256) void k_linact_join(const float* __restrict__ part, int splits, int64_t M, int64_t N,
                                                      const LaEpi<OT> e) {
-  constexpr int V = Elem<OT>::VEC;
-  __shared__ __align__(16) float sums[8][32][V];
+  constexpr int V = Elem<OT>::VEC, PIECES = 256 / LANES;
+  __shared__ __align__(16) float sums[LANES > 1 ? LANES : 1][PIECES][V];
   const int64_t per_row = (N + V - 1) / V, total = M * per_row;
-  const int piece = threadIdx.x & 31, lane = threadIdx.x >> 5;
-  for (int64_t t0 = (int64_t)blockIdx.x * 32; t0 < total; t0 += (int64_t)gridDim.x * 32) {
+  const int piece = threadIdx.x % PIECES, lane = threadIdx.x / PIECES;
+  for (int64_t t0 = (int64_t)blockIdx.x * PIECES; t0 < total; t0 += (int64_t)gridDim.x * PIECES) {
     const int64_t t = t0 + piece, m = t / per_row, n = t % per_row * V;
     const int left = (int)(N - n < V ? N - n : V);
     float z[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) z[k] = 0.f;
     if (t < total)
-      for (int s = lane; s < splits; s += 8) {
+      for (int s = lane; s < splits; s += LANES) {
         const float* row = part + ((int64_t)s * M + m) * N + n;
 #pragma unroll
         for (int i = 0; i < V; i += 4) {
+          if (i >= left) continue;
           const f32x4 v = ffn_load(row, i, left);
 #pragma unroll
           for (int k = 0; k < 4; ++k) z[i + k] += v[k];
         }
       }
+    if (LANES > 1) {
 #pragma unroll
-    for (int i = 0; i < V; i += 4) *reinterpret_cast<f32x4*>(&sums[lane][piece][i]) = f32x4{z[i], z[i + 1], z[i + 2], z[i + 3]};
-    __syncthreads();
-    if (lane == 0 && t < total) {
-      const int parts = splits < 8 ? splits : 8;
-      for (int s = 1; s < parts; ++s)
+      for (int i = 0; i < V; i += 4) *reinterpret_cast<f32x4*>(&sums[lane][piece][i]) = f32x4{z[i], z[i + 1], z[i + 2], z[i + 3]};
+      __syncthreads();
+      if (lane == 0)
+        for (int s = 1; s < LANES; ++s)
 #pragma unroll
-        for (int k = 0; k < V; ++k) z[k] += sums[s][piece][k];
-      la_finish<V>(e, m, n, N, z);
+          for (int k = 0; k < V; ++k) z[k] += sums[s][piece][k];
+      __syncthreads();
     }
-    __syncthreads();
+    if (lane == 0 && t < total) la_finish<V>(e, m, n, N, z);
   }
 }
 
@@ -822,7 +824,10 @@ int la_product(const hotk_linear_args& a, void* ws, size_t nws, hipStream_t st) 
                        : la_run<IT, OT, TA, TB, 64, 64, 4, 1>(g, s.splits, st);
   if (rc == HOTK_OK && need) {
     const int64_t work = a.M * la_div(a.N, Elem<OT>::VEC);
-    hipLaunchKernelGGL(k_linact_join<OT>, dim3(hotk_grid(work, 32, 256 * 32)), dim3(256), 0, st, (const float*)ws, s.splits, a.M, a.N, g.e);
+    if (s.splits <= 4)
+      hipLaunchKernelGGL((k_linact_join<OT, 1>), dim3(hotk_grid(work, 256)), dim3(256), 0, st, (const float*)ws, s.splits, a.M, a.N, g.e);
+    else
+      hipLaunchKernelGGL((k_linact_join<OT, 8>), dim3(hotk_grid(work, 32, 256 * 32)), dim3(256), 0, st, (const float*)ws, s.splits, a.M, a.N, g.e);
     rc = hotk_launch_status();
   }
   return rc;
