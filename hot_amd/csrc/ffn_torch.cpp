@@ -1,7 +1,7 @@
 // Host side of the feed-forward operators (hot_amd/ffn.py): argument checks, result and workspace tensors, autograd nodes, and the
-// launches through the C entries of libhotk.so.  In C++ because a call is a few microseconds of GPU work at the small end: the
-// same steps in Python (ctypes arguments, a Python autograd function) cost 16 us a forward call and 160 us a call with its
-// gradients, against 5 and 25 here.
+// launches through the C entries of libhotk.so.  In C++ because a call is a few microseconds of GPU work at the small end: with
+// the same steps in Python (ctypes arguments, a Python autograd function) a norm of one token took 22 us a call and one with
+// its gradients 160, against 4.7 and 55 here, of which torch's own engine takes 31.
 //
 // The entries' addresses come from Python's loaded library (bind), so both bindings run the same build of it; with timing on
 // (_lib.timing_begin) every launch is reported to the same hook as Python's own.

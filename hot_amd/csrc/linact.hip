@@ -22,6 +22,10 @@
 // matrix instructions: by then every fragment of the stage is in registers and the next stage has landed, so behind the
 // barrier the DMA of the step after next starts and the next step's first fragments are read while matrix instructions run.
 //
+// Measured (large library products reach 1 354 TFLOP/s in bf16, 2 748 in e4m3, 153 in fp32 here): 8 192^3 bf16 807 us =
+// 1 362 TFLOP/s, 8 192^3 e4m3 389 us = 2 823; 16 384 x 4 096 x 1 024 bf16 129 us = 1 066 (with bias, gelu and slopes 184), its
+// dx 111 us = 1 238, its dw 135 us = 1 018; 8 192 x 2 048 x 4 096 e4m3 62 us = 2 200; 4 096 x 4 096 x 1 024 fp32 254 us = 135.
+//
 // For training, 16-bit types keep f'(z) as a 16-bit fixed-point number in steps of 2^-14 (|f'| < 1.13): its error of 2^-15
 // is far below the rounding of dz, where z rounded to the type would add as much as that rounding again, and the backward
 // pass needs no transcendental.  fp32 keeps z.
