@@ -49,6 +49,7 @@ constexpr float LA_SLOPE_STEP = 0x1p-14f;
 constexpr int LA_SLOPE_NAN = -32768;
 constexpr float LA_LEAK = 0.01f;
 constexpr int LA_MAX_SPLIT = 16;
+constexpr int64_t LA_MAX_GRID = 1 << 23;           // workgroups of up to 512 threads: a launch holds fewer than 2^32 threads
 
 __device__ __align__(16) const uint32_t la_zeros[4] = {0, 0, 0, 0};   // what lies past the end of a contraction
 
@@ -781,6 +782,7 @@ LaShape la_shape(const hotk_linear_args& a);
 
 template <class IT, class OT, int MB>
 int la_run_few(const LaTile<OT>& g, hipStream_t st) {
+  if (la_div(g.N, 16) >= LA_MAX_GRID) return HOTK_ETOOLARGE;
   hipLaunchKernelGGL((k_linact_few<IT, OT, MB>), dim3((unsigned)la_div(g.N, 16)), dim3(512), 0, st, g);
   return hotk_launch_status();
 }
@@ -800,6 +802,7 @@ int la_run(LaTile<OT>& g, int splits, hipStream_t st) {
       asked.fetch_or(bit, std::memory_order_relaxed);
     }
   }
+  if (la_div(g.M, BM) * la_div(g.N, BN) >= LA_MAX_GRID) return HOTK_ETOOLARGE;
   g.tiles_m = (int)la_div(g.M, BM);
   g.tiles_n = (int)la_div(g.N, BN);
   hipLaunchKernelGGL(kernel, dim3((unsigned)(g.tiles_m * g.tiles_n), (unsigned)splits), dim3(64 * WM * WN), LDS, st, g);
@@ -870,7 +873,7 @@ int la_check(const hotk_linear_args& a) {
     HOTK_CHECK_ARG(((uintptr_t)a.x_scale) % 4 == 0 && ((uintptr_t)a.w_scale) % 4 == 0);
   }
   // 32-bit offsets inside a tile, 32-bit tile and step counts
-  if (a.ld_x * e > (1 << 23) || a.ld_w * e > (1 << 23) || la_div(a.M, 64) * la_div(a.N, 64) > (1ll << 30) || la_div(a.N, 16) > (1ll << 30) || la_div(a.K * e, 128) > (1ll << 30))
+  if (a.ld_x * e > (1 << 23) || a.ld_w * e > (1 << 23) || la_div(a.M, 64) * la_div(a.N, 64) > (1ll << 30) || la_div(a.K * e, 128) > (1ll << 30))
     return HOTK_ETOOLARGE;
   return HOTK_OK;
 }
@@ -927,7 +930,7 @@ extern "C" int hotk_linear_dz(const void* in, int64_t ld_in, const void* save, i
   int cg_log = 0;
   while (cg_log < 5 && (1 << cg_log) < pieces) ++cg_log;
   const int64_t across = la_div(pieces, 1 << cg_log);
-  if (across > (1 << 20) || rows > (1 << 30)) return HOTK_ETOOLARGE;
+  if (across * down >= 2 * LA_MAX_GRID || rows > (1 << 30)) return HOTK_ETOOLARGE;
   ffn_dispatch(type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     hipLaunchKernelGGL(k_linact_dz<T>, dim3((unsigned)(across * down)), dim3(256), 0, (hipStream_t)stream, (const T*)in, ld_in, save, act,

@@ -463,6 +463,7 @@ extern "C" int hotk_sum_partials(const float* partial, int64_t n, int64_t D, voi
   HOTK_CHECK_ARG(n >= 0 && D >= 0);
   if (!ffn_type_ok(type)) return HOTK_EUNSUPPORTED;
   if (D == 0) return HOTK_OK;
+  if (D > (1 << 25)) return HOTK_ETOOLARGE;      // (a launch holds fewer than 2^32 threads)
   HOTK_CHECK_ARG(out && (partial || n == 0) && ffn_elem_aligned(out, type));
   const dim3 grid((unsigned)((D + 15) / 16)), block(1024);
   ffn_dispatch(type, [&](auto* tag) {

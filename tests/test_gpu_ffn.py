@@ -231,6 +231,99 @@ def test_empty_batches(R):
     assert ops.linear_act_quantized(q, s, wq, ws, out_dtype=torch.float32).shape == (R, 8)
 
 
+def test_offsets_past_32_bits():
+    """more than 2^31 elements: the last rows equal the same rows in a small call"""
+    from hot_amd import ops
+    R, D, dt = 1100000, 2048, torch.bfloat16
+    tail = slice(R - 70, R)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(R, D, generator=g, device=DEV, dtype=dt)
+    w = rnd(1, D, dt=dt)
+    y, h = ops.rms_norm(x, w, x)
+    ys, hs = ops.rms_norm(x[tail], w, x[tail])
+    assert torch.equal(y[tail], ys) and torch.equal(h[tail], hs)
+    del y, h
+    q, s = ops.quantize_rows(x)
+    qs, ss = ops.quantize_rows(x[tail])
+    assert torch.equal(q[tail].float(), qs.float()) and torch.equal(s[tail], ss)
+    del q, s
+    W = rnd(2, D, 24, dt=dt, scale=0.2)
+    z = ops.linear_act(x[:, :24], W, act='relu', residual=x)                # read at a stride, 2^31 results
+    assert torch.equal(z[tail], ops.linear_act(x[tail, :24].contiguous(), W, act='relu', residual=x[tail]))
+    del z
+    leaf = x[:, 24:48].detach().requires_grad_(True)
+    dx, = torch.autograd.grad(ops.linear_act(leaf, W), leaf, x)
+    want = x[tail].double() @ W.double()                                    # (a small call may split its sum: not bit for bit)
+    hold('dx', dx[tail], want, half_step(dt) * want.abs() + (D + 8) * E * (x[tail].double().abs() @ W.double().abs()))
+    V = rnd(3, 16, D, dt=dt, scale=0.02).requires_grad_(True)
+    dV, = torch.autograd.grad(ops.linear_act(x, V), V, rnd(4, R, 16, dt=dt))
+    ref = (rnd(4, R, 16, dt=dt)[-1000:].double().t() @ x[-1000:].double())
+    part, = torch.autograd.grad(ops.linear_act(x[-1000:], V), V, rnd(4, R, 16, dt=dt)[-1000:].contiguous())
+    assert dV.isfinite().all() and float((part.double() - ref).norm() / ref.norm()) < half_step(dt)
+
+
+@pytest.mark.parametrize('dt', TYPES)
+def test_one_tensor_in_two_places(dt):
+    """the stream as its own residual, the weight as the rows: gradients add up"""
+    from hot_amd import ops
+    x, w = rnd(400, 30, 64, dt=dt).requires_grad_(True), rnd(401, 64, dt=dt)
+    dy, dh = rnd(402, 30, 64, dt=dt), rnd(403, 30, 64, dt=dt)
+    both, = torch.autograd.grad(ops.rms_norm(x, w, x), x, (dy, dh))
+    a, b = x.detach().requires_grad_(True), x.detach().requires_grad_(True)
+    ga, gb = torch.autograd.grad(ops.rms_norm(a, w, b), (a, b), (dy, dh))
+    assert torch.equal(both, ga + gb)
+    W = rnd(404, 40, 64, dt=dt).requires_grad_(True)
+    dz = rnd(405, 40, 40, dt=dt)
+    both, = torch.autograd.grad(ops.linear_act(W, W, act='gelu'), W, dz)
+    a, b = W.detach().requires_grad_(True), W.detach().requires_grad_(True)
+    ga, gb = torch.autograd.grad(ops.linear_act(a, b, act='gelu'), (a, b), dz)
+    assert torch.equal(both, ga + gb)
+    x.grad = None
+    y, h = ops.rms_norm(x, w, x)
+    y.backward(dy)                                   # only one of the two outputs has a gradient
+    only_y = x.grad.clone()
+    y, h = ops.rms_norm(a_ := x.detach().requires_grad_(True), w, a_)
+    g2, = torch.autograd.grad((y, h), a_, (dy, torch.zeros_like(h)))
+    assert torch.equal(only_y, g2)
+    y, h = ops.rms_norm(x, w, x)
+    g3, = torch.autograd.grad(h, x, dh)
+    assert torch.equal(g3, dh + dh)
+
+
+def test_calls_from_several_threads():
+    """forward and backward from four threads on streams of their own"""
+    import threading
+    from hot_amd import ops
+    p = block_params(136, 264, 90, torch.bfloat16, seed=410)
+    xs = [rnd(420 + i, 90, 136, dt=torch.bfloat16) for i in range(4)]
+    dy = rnd(430, 90, 136, dt=torch.bfloat16)
+
+    def step(x):
+        leaves = [t.detach().requires_grad_(True) for t in [x] + list(p.values())]
+        y = block(ops, leaves[0], dict(zip(p, leaves[1:])))
+        return [y.detach()] + list(torch.autograd.grad(y, leaves, dy))
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(10):
+                    got[i] = step(xs[i])
+            s.synchronize()
+        except Exception as e:      # noqa: BLE001 (shown by the assertion below)
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not errors, errors
+    assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
 def test_wide_rows():
     from hot_amd import ops
     for dt in TYPES:
