@@ -768,7 +768,7 @@ LaShape la_shape(int64_t M, int64_t N, int64_t K, int type, int out_type, int fl
       const int64_t kper = la_div(ktiles, s), splits = la_div(ktiles, kper);
       const float q = (float)std::ceil(tiles * splits / 256.);
       float t = q * c.end + kper * std::max(lat, sat * q);
-      if (splits > 1) t += 3.5f + splits * (float)M * N * 4.f / 3e6f;       // the join: a launch, and the parts written and read
+      if (splits > 1) t += 6.f + splits * (float)M * N * 4.f / 3e6f;       // the join: a launch on either side, and the parts written and read
       if (t < least) {
         least = t;
         best = {c.bm, c.bn, (int)splits};
@@ -878,9 +878,9 @@ int la_check(const hotk_linear_args& a) {
   return HOTK_OK;
 }
 
-// rows of a block of hotk_linear_dz: all of up to 64 (one block: its sums are the result), else 16, and more where that would be
-// over 512 blocks
-int64_t la_dz_rows(int64_t R) { return R <= 64 ? 64 : la_div(la_div(R, 512), 16) * 16; }
+// rows of a block of hotk_linear_dz: all of up to 1024 (one block: its sums are the result, and a launch is saved), else 16, and
+// more where that would be over 512 blocks
+int64_t la_dz_rows(int64_t R) { return R <= 1024 ? 1024 : la_div(la_div(R, 512), 16) * 16; }
 
 }  // namespace
 
@@ -927,8 +927,8 @@ extern "C" int hotk_linear_dz(const void* in, int64_t ld_in, const void* save, i
   if (R == 0) return HOTK_OK;
   HOTK_CHECK_ARG(in);
   const int64_t pieces = la_div(out ? ld_out : C, 16 / ffn_bytes(type)), rows = la_dz_rows(R), down = la_div(R, rows);
-  int cg_log = 0;
-  while (cg_log < 5 && (1 << cg_log) < pieces) ++cg_log;
+  int cg_log = 0;                          // 32 pieces side by side; 4 where one block has many rows
+  while (cg_log < (rows >= 1024 && R > 64 ? 2 : 5) && (1 << cg_log) < pieces) ++cg_log;
   const int64_t across = la_div(pieces, 1 << cg_log);
   if (across * down >= 2 * LA_MAX_GRID || rows > (1 << 30)) return HOTK_ETOOLARGE;
   ffn_dispatch(type, [&](auto* tag) {

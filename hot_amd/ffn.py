@@ -22,11 +22,8 @@ def _ext():
     return _binding
 
 
-def _call(name, *args):
-    try:
-        return getattr(_binding or _ext(), name)(*args)
-    except TypeError as e:
-        raise HotkError(f'{name}: an argument is not of the documented kind ({str(e).splitlines()[0]})') from None
+def _wrong(name, e):
+    return HotkError(f'{name}: an argument is not of the documented kind ({str(e).splitlines()[0]})')
 
 
 def rms_norm(x, weight, residual=None, eps=1e-6, kind=None, keep=KEEP_VALID):
@@ -36,21 +33,30 @@ def rms_norm(x, weight, residual=None, eps=1e-6, kind=None, keep=KEEP_VALID):
     x, residual [..., D], weight [D], one type (fp32, bf16, fp16), D <= 32768.  kind (uint8, one per row: a plan's `kind` or
     `nkind`) and keep: rows that keep leaves out are not read, and are zero in y, h and the gradients.  Differentiable in x,
     weight and residual."""
-    return _call('rms_norm', x, weight, residual, eps, kind, keep)
+    try:
+        return (_binding or _ext()).rms_norm(x, weight, residual, eps, kind, keep)
+    except TypeError as e:
+        raise _wrong('rms_norm', e) from None
 
 
 def rms_norm_quantized(x, weight, residual=None, eps=1e-6, kind=None, keep=KEEP_VALID):
     """rms_norm with y in 8 bits for a product of 8-bit operands (linear_act_quantized): (q, scale), with a residual (q, scale,
     h).  scale[row] = max(max|y| / 448, 2^-126) in fp32, q = e4m3(y / scale), torch.float8_e4m3fn, from y in 32 bits.  A row
     that holds an infinity or NaN comes out with a scale that is one.  No gradient."""
-    return _call('rms_norm_quantized', x, weight, residual, eps, kind, keep)
+    try:
+        return (_binding or _ext()).rms_norm_quantized(x, weight, residual, eps, kind, keep)
+    except TypeError as e:
+        raise _wrong('rms_norm_quantized', e) from None
 
 
 def quantize_rows(x):
     """(q, scale): rows of x [..., D] (fp32, bf16, fp16; D <= 32768) to torch.float8_e4m3fn with one fp32 scale each, scale =
     max(max|x| / 448, 2^-126), q = e4m3(x / scale): the operands of linear_act_quantized, weights ([N, K], a scale per output
     column) as well as activations.  A row that holds an infinity or NaN comes out with a scale that is one.  No gradient."""
-    return _call('quantize_rows', x)
+    try:
+        return (_binding or _ext()).quantize_rows(x)
+    except TypeError as e:
+        raise _wrong('quantize_rows', e) from None
 
 
 def linear_act(x, weight, bias=None, act='none', residual=None):
@@ -60,7 +66,10 @@ def linear_act(x, weight, bias=None, act='none', residual=None):
 
     Rows that start at 16-byte boundaries and hold whole 16-byte pieces (K a multiple of 8, of 4 in fp32) are read in place;
     others are copied once with zeros behind them.  Rows of up to 8 MiB, else HotkError."""
-    return _call('linear_act', x, weight, bias, act, residual)
+    try:
+        return (_binding or _ext()).linear_act(x, weight, bias, act, residual)
+    except TypeError as e:
+        raise _wrong('linear_act', e) from None
 
 
 def linear_act_quantized(xq, x_scale, wq, w_scale, bias=None, act='none', residual=None, out_dtype=torch.bfloat16):
@@ -69,4 +78,7 @@ def linear_act_quantized(xq, x_scale, wq, w_scale, bias=None, act='none', residu
     and y in out_dtype (bf16, fp16, fp32).  For an fp32 result products are added up in 32 bits; for 16-bit ones the 8-bit
     matrix instruction adds them by eights to 2^-13 of the largest of the eight, and the eights in 32 bits.  K a multiple of 16
     is read in place.  No gradient."""
-    return _call('linear_act_quantized', xq, x_scale, wq, w_scale, bias, act, residual, out_dtype)
+    try:
+        return (_binding or _ext()).linear_act_quantized(xq, x_scale, wq, w_scale, bias, act, residual, out_dtype)
+    except TypeError as e:
+        raise _wrong('linear_act_quantized', e) from None

@@ -94,7 +94,7 @@ def test_backward_entries_refuse():
     assert dz(R=0) == 0
     assert dz(i=NULL) == EINVAL and dz(ld=7) == EINVAL and dz(ld_o=7) == EINVAL and dz(out=NULL) == EINVAL and dz(C=0, ld=0, ld_o=0) == EINVAL
     assert dz(act=3) == EINVAL and dz(act=6, save=SOME) == EINVAL and dz(i=ctypes.c_void_p(4097)) == EINVAL
-    assert dz(total=SOME, R=1000) == EINVAL and dz(total=SOME, part=SOME) == EINVAL          # a total of one block only
+    assert dz(total=SOME, R=2000) == EINVAL and dz(total=SOME, part=SOME) == EINVAL          # a total of one block only
     assert dz(ty=5) == EUNSUPPORTED and dz(ty=3) == EUNSUPPORTED
     n = ctypes.c_int64()
     for R in (0, 1, 16, 17, 8191, 8193, 10 ** 7):
