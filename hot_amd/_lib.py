@@ -120,7 +120,7 @@ class LinearArgs(ctypes.Structure):
     """mirror of hotk_linear_args (include/hotk.h)"""
     _fields_ = [('M', _L), ('N', _L), ('K', _L), ('x', _P), ('ld_x', _L), ('w', _P), ('ld_w', _L), ('bias', _P), ('res', _P),
                 ('ld_res', _L), ('y', _P), ('ld_y', _L), ('save', _P), ('x_scale', _P), ('w_scale', _P),
-                ('type', ctypes.c_int32), ('out_type', ctypes.c_int32), ('act', ctypes.c_int32), ('flags', ctypes.c_int32)]
+                ('type', ctypes.c_int32), ('out_type', ctypes.c_int32), ('act', ctypes.c_int32), ('flags', ctypes.c_int32), ('x_lo', _P)]
 
 
 _SIGNATURES.update({
@@ -134,7 +134,7 @@ _SIGNATURES.update({
     'hotk_linear_workspace_bytes': [ctypes.POINTER(LinearArgs), ctypes.POINTER(_S)],
     'hotk_linear_act': [ctypes.POINTER(LinearArgs), _P, _S, _P],
     'hotk_linear_dz_partials': [_L, ctypes.POINTER(_L)],
-    'hotk_linear_dz': [_P, _L, _P, _I, _P, _L, _P, _P, _L, _L, _I, _P],
+    'hotk_linear_dz': [_P, _L, _P, _I, _P, _P, _L, _P, _P, _L, _L, _I, _P],
     'hotk_pad_rows': [_P, _L, _P, _L, _L, _L, _P],
 })
 EXPORTS = sorted(list(_SIGNATURES) + ['hotk_strerror', 'hotk_version'])

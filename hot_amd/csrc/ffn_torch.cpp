@@ -322,6 +322,7 @@ Rows padded(const Rows& in, int64_t C) {   // itself where it is whole, else a c
 struct Extras {
   Tensor bias, save, x_scale, w_scale;
   Rows res;
+  const void* x_lo = nullptr;
   int act = HOTK_ACT_NONE, flags = 0;
 };
 // epilogue(x w^T) [M, N] as a new tensor of this shape (no view: the caller may go on in place), copies of operands
@@ -340,7 +341,7 @@ Tensor product(const Rows& x, const Rows& w, int64_t M, int64_t N, int64_t K, at
   a.y = y.data_ptr(); a.ld_y = N;
   a.save = out(e.save);
   a.x_scale = (const float*)out(e.x_scale); a.w_scale = (const float*)out(e.w_scale);
-  a.type = ty; a.out_type = type_of(type); a.act = e.act; a.flags = e.flags;
+  a.type = ty; a.out_type = type_of(type); a.act = e.act; a.flags = e.flags; a.x_lo = e.x_lo;
   if (x.zeros && (w.zeros || (a.flags & HOTK_LINEAR_W_DOWN))) a.flags |= HOTK_LINEAR_PADDED;
   size_t need = 0;
   int rc = L.linear_workspace_bytes(&a, &need);
@@ -450,9 +451,13 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         // one pass over dy: dz where it is not dy itself, and its column sums
         Rows dz = gs;
         const bool itself = act == HOTK_ACT_NONE && whole(gs, N);
+        // dz is rounded to the type for the products, which adds as much error as the result's own rounding.  Where the products
+        // hide behind the launches around them the rest goes in too: up to 2^25 multiplications (1 to 5 us of the two products'
+        // 10 to 20, beside 50 that the host takes; at 2^28 it would be 7 of 14)
+        const bool two_parts = act != HOTK_ACT_NONE && type != at::kFloat && (double)M * N * K <= 33554432.;
         if ((wants & 3) && !itself) {
           const int64_t ld = up(N, x.element_size());
-          dz = {like(x, {M, ld}, type), ld, M, true};
+          dz = {like(x, {two_parts ? 2 * M : M, ld}, type), ld, M, true};
         }
         Tensor part;
         if (wants & 4) {
@@ -462,9 +467,10 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
           if (n > 1) part = like(x, {n, N}, at::kFloat);
         }
         const bool write = (wants & 3) && !itself;
+        void* lo = write && two_parts ? (char*)dz.t.data_ptr() + M * dz.ld * x.element_size() : nullptr;
         if (write || db.defined())
           launch("hotk_linear_dz", M * N * x.element_size() * (1 + write + (act != HOTK_ACT_NONE)), [&] {
-            return L.linear_dz(gs.p(), gs.ld, out(save), act, write ? dz.t.data_ptr() : nullptr, dz.ld, (float*)out(part), part.defined() ? nullptr : out(db),
+            return L.linear_dz(gs.p(), gs.ld, out(save), act, write ? dz.t.data_ptr() : nullptr, lo, dz.ld, (float*)out(part), part.defined() ? nullptr : out(db),
                                M, N, ty, stream_of(x));
           });
         if (part.defined())
@@ -472,6 +478,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
             return L.sum_partials(part.const_data_ptr<float>(), part.size(0), N, db.data_ptr(), ty, stream_of(x));
           });
         Extras e;
+        e.x_lo = lo;
         if (wants & 1) {
           e.flags = HOTK_LINEAR_W_DOWN;
           dx = product(dz, padded(ld[1] ? Rows{weight, ld[1], N, true} : rows(weight), K), M, K, N, shape, type, e);

@@ -236,6 +236,8 @@ struct LaTile {
   int64_t lda, ldb;              // bytes per row
   int64_t M, N, K;
   int ktiles, kper;              // 128-byte steps, and how many of them a split takes
+  int wrap;                      // steps of the contraction: from here on x_lo, `low` bytes behind x, takes x's place
+  int64_t low;
   int tiles_m, tiles_n;
   float* part;                   // [splits][M][N] bare products, where there is more than one split
   LaEpi<OT> e;
@@ -387,8 +389,8 @@ struct LaFeed {
       off[i] = (uint32_t)(row * ld) + chunk * 16;
     }
   }
-  __device__ __forceinline__ void issue(int kt, int64_t K, uint32_t dst) const {
-    const char* at = base + (T ? (int64_t)kt * S::STEP * ld : (int64_t)kt * 128);
+  __device__ __forceinline__ void issue(int kt, int64_t K, uint32_t dst, int64_t shift) const {
+    const char* at = base + shift + (T ? (int64_t)kt * S::STEP * ld : (int64_t)kt * 128);
     if ((int64_t)(kt + 1) * S::STEP <= K) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) la_dma(at, off[i], dst + (wave + NW * i) * 1024);
@@ -423,8 +425,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_linact_tile(const LaTile<OT> g
   const LaFeed<IT, TA, BM, NW> fa(g.a, g.lda, m0, g.M, wave, lane);
   const LaFeed<IT, TB, BN, NW> fb(g.b, g.ldb, n0, g.N, wave, lane);
   auto issue = [&](int kt, int stage) {
-    fa.issue(kt, g.K, lds0 + stage * XS);
-    fb.issue(kt, g.K, lds0 + W0 + stage * WS);
+    const bool lo = kt >= g.wrap;
+    const int k = lo ? kt - g.wrap : kt;
+    fa.issue(k, g.K, lds0 + stage * XS, lo ? g.low : 0);
+    fb.issue(k, g.K, lds0 + W0 + stage * WS, 0);
   };
 
   f32x4 acc[MF][NF];
@@ -657,12 +661,12 @@ __global__ __launch_bounds__(512) void k_linact_few(const LaTile<OT> g) {
 
 // ---- backward: dz and its column sums; rows padded to whole pieces ---------------------------------------------------------
 // v = in * slope over a block of `rows` rows: out [R, ld_out] with zeros from C on, partial [block][C] the block's column sums, or
-// total [C] where there is one block.
+// total [C] where there is one block.  out_lo: what out's rounding left, so that out + out_lo is v to the square of a half step
 // A thread owns one 16-byte piece of columns and every (256 / cg)th row of the block; cg (a power of two) pieces go side by side
 template <class T>
 __global__ __launch_bounds__(256) void k_linact_dz(const T* __restrict__ in, int64_t ld_in, const void* __restrict__ save, int act,
-                                                   T* __restrict__ out, int64_t ld_out, float* __restrict__ partial,
-                                                   T* __restrict__ total, int64_t R, int64_t C, int rows, int cg_log, unsigned across) {
+                                                   T* __restrict__ out, T* __restrict__ out_lo, int64_t ld_out,
+                                                   float* __restrict__ partial, T* __restrict__ total, int64_t R, int64_t C, int rows, int cg_log, unsigned across) {
   using E = Elem<T>;
   using FV = typename E::fvec;
   __shared__ FV sums[256];
@@ -696,7 +700,16 @@ __global__ __launch_bounds__(256) void k_linact_dz(const T* __restrict__ in, int
         }
         s += v;
       }
-      if (out && room > 0) ffn_store(out + r * ld_out + c, 0, room, v);
+      if (out && room > 0) {
+        ffn_store(out + r * ld_out + c, 0, room, v);
+        if (out_lo) {
+          const FV hi = __builtin_convertvector(__builtin_convertvector(v, typename E::vec), FV);
+          FV lo;
+#pragma unroll
+          for (int k = 0; k < E::VEC; ++k) lo[k] = hi[k] - hi[k] == 0.f ? v[k] - hi[k] : 0.f;     // (an infinity leaves nothing)
+          ffn_store(out_lo + r * ld_out + c, 0, room, lo);
+        }
+      }
     }
   }
   if (partial || total) {
@@ -743,13 +756,13 @@ int64_t la_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct LaShape { int bm, bn, splits; };      // bn 16: k_linact_few, bm / 16 blocks of rows
 struct LaCost { int bm, bn; float sat, lat, end; };
 const LaCost LA_COSTS[] = {{256, 256, 1.58f, 1.58f, 6.f}, {128, 128, 0.42f, 0.69f, 3.f}, {64, 128, 0.26f, 0.39f, 1.2f}, {64, 64, 0.16f, 0.32f, 0.7f}};
-LaShape la_shape(int64_t M, int64_t N, int64_t K, int type, int out_type, int flags, bool whole) {
-  const int64_t ktiles = la_div(K * ffn_bytes(type), 128);
+LaShape la_shape(int64_t M, int64_t N, int64_t K, int type, int out_type, int flags, bool whole, int parts) {
+  const int64_t ktiles = la_div(K * ffn_bytes(type), 128) * parts;
   const bool wide = type == HOTK_E4M3 && out_type == HOTK_F32;
   const float mfma = type == HOTK_F32 ? 8.f : wide ? 2.f : 1.f;
   LaShape best{64, 64, 1};
   float least = 1e30f;
-  if (M <= 64 && flags == 0) {               // k_linact_few: 8.6 TB/s in all, 50 GB/s a compute unit, its matrix work beside that
+  if (M <= 64 && flags == 0 && parts == 1) {     // k_linact_few: 8.6 TB/s in all, 50 GB/s a compute unit, its matrix work beside that
     const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
     const float wgs = (float)la_div(N, 16), bytes = ktiles * 128.f * 16 * (1 + mb);
     // (rows in no whole pieces: the tiles would need two copies first)
@@ -812,7 +825,7 @@ int la_run(LaTile<OT>& g, int splits, hipStream_t st) {
 template <class IT, class OT, bool TA, bool TB>
 int la_product(const hotk_linear_args& a, void* ws, size_t nws, hipStream_t st) {
   const int e = ffn_bytes(a.type);
-  const int64_t ktiles = la_div(a.K * e, 128);
+  const int64_t steps = la_div(a.K * e, 128), ktiles = a.x_lo ? 2 * steps : steps;
   const LaShape s = la_shape(a);
   const size_t need = s.splits > 1 ? (size_t)s.splits * a.M * a.N * 4 : 0;
   if (nws < need || (need && !ws)) return HOTK_EWORKSPACE;
@@ -820,6 +833,8 @@ int la_product(const hotk_linear_args& a, void* ws, size_t nws, hipStream_t st) 
   g.a = (const char*)a.x; g.b = (const char*)a.w;
   g.lda = a.ld_x * e; g.ldb = a.ld_w * e;
   g.M = a.M; g.N = a.N; g.K = a.K;
+  g.wrap = (int)steps;
+  g.low = a.x_lo ? (const char*)a.x_lo - (const char*)a.x : 0;
   g.ktiles = (int)ktiles; g.kper = (int)la_div(ktiles, s.splits);
   g.part = need ? (float*)ws : nullptr;
   g.e = {(const OT*)a.bias, (const OT*)a.res, a.ld_res, (OT*)a.y, a.ld_y, a.save, a.x_scale, a.w_scale, a.act};
@@ -848,7 +863,7 @@ bool la_whole(const hotk_linear_args& a) {
   return a.ld_x >= la_div(row_x, m) * m && a.ld_w >= la_div(row_w, m) * m && (a.ld_x * e) % 16 == 0 && (a.ld_w * e) % 16 == 0 &&
          hotk_aligned16(a.x) && hotk_aligned16(a.w);
 }
-LaShape la_shape(const hotk_linear_args& a) { return la_shape(a.M, a.N, a.K, a.type, a.out_type, a.flags & (HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN), la_whole(a)); }
+LaShape la_shape(const hotk_linear_args& a) { return la_shape(a.M, a.N, a.K, a.type, a.out_type, a.flags & (HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN), la_whole(a), a.x_lo ? 2 : 1); }
 
 int la_check(const hotk_linear_args& a) {
   HOTK_CHECK_ARG(a.M >= 0 && a.N > 0 && a.K > 0);
@@ -868,6 +883,7 @@ int la_check(const hotk_linear_args& a) {
     HOTK_CHECK_ARG(ffn_elem_aligned(a.x, a.type) && ffn_elem_aligned(a.w, a.type));
     // the tiles read rows in whole, aligned 16-byte pieces (the caller pads others: hotk_pad_rows)
     if (!la_whole(a) && la_shape(a).bn != 16) return HOTK_EUNSUPPORTED;
+    if (a.x_lo && (!hotk_aligned16(a.x_lo) || a.type == HOTK_E4M3)) return HOTK_EUNSUPPORTED;
     HOTK_CHECK_ARG(ffn_elem_aligned(a.y, a.out_type) && ffn_elem_aligned(a.bias, a.out_type) && ffn_elem_aligned(a.res, a.out_type));
     HOTK_CHECK_ARG(((uintptr_t)a.save) % (a.out_type == HOTK_F32 ? 4 : 2) == 0);
     HOTK_CHECK_ARG(((uintptr_t)a.x_scale) % 4 == 0 && ((uintptr_t)a.w_scale) % 4 == 0);
@@ -916,13 +932,14 @@ extern "C" int hotk_linear_dz_partials(int64_t R, int64_t* n_partials) {
   return HOTK_OK;
 }
 
-extern "C" int hotk_linear_dz(const void* in, int64_t ld_in, const void* save, int act, void* out, int64_t ld_out, float* partial,
-                              void* total, int64_t R, int64_t C, int type, void* stream) {
+extern "C" int hotk_linear_dz(const void* in, int64_t ld_in, const void* save, int act, void* out, void* out_lo, int64_t ld_out,
+                              float* partial, void* total, int64_t R, int64_t C, int type, void* stream) {
   HOTK_CHECK_ARG(R >= 0 && C > 0 && ld_in >= C && (!out || ld_out >= C) && (out || partial || total));
+  HOTK_CHECK_ARG(!out_lo || out);
   HOTK_CHECK_ARG(!total || (!partial && R <= la_dz_rows(R)));
   HOTK_CHECK_ARG(act >= HOTK_ACT_NONE && act <= HOTK_ACT_SILU && (act == HOTK_ACT_NONE || save || R == 0));
   if (!ffn_type_ok(type)) return HOTK_EUNSUPPORTED;
-  HOTK_CHECK_ARG(ffn_elem_aligned(in, type) && ffn_elem_aligned(out, type) && ffn_elem_aligned(total, type) && ((uintptr_t)save) % (type == HOTK_F32 ? 4 : 2) == 0 &&
+  HOTK_CHECK_ARG(ffn_elem_aligned(in, type) && ffn_elem_aligned(out, type) && ffn_elem_aligned(out_lo, type) && ffn_elem_aligned(total, type) && ((uintptr_t)save) % (type == HOTK_F32 ? 4 : 2) == 0 &&
                  ((uintptr_t)partial) % 4 == 0);
   if (R == 0) return HOTK_OK;
   HOTK_CHECK_ARG(in);
@@ -934,7 +951,7 @@ extern "C" int hotk_linear_dz(const void* in, int64_t ld_in, const void* save, i
   ffn_dispatch(type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     hipLaunchKernelGGL(k_linact_dz<T>, dim3((unsigned)(across * down)), dim3(256), 0, (hipStream_t)stream, (const T*)in, ld_in, save, act,
-                       (T*)out, ld_out, partial, (T*)total, R, C, (int)rows, cg_log, (unsigned)across);
+                       (T*)out, (T*)out_lo, ld_out, partial, (T*)total, R, C, (int)rows, cg_log, (unsigned)across);
   });
   return hotk_launch_status();
 }

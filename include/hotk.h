@@ -556,15 +556,17 @@ typedef struct {
   const float* x_scale;
   const float* w_scale;
   int32_t type, out_type, act, flags;
+  const void* x_lo;   /* NULL, or a second part of x, of its layout, type and alignment: z = (x + x_lo) w^T + bias */
 } hotk_linear_args;
 int hotk_linear_workspace_bytes(const hotk_linear_args* args, size_t* bytes);       /* for exactly these arguments */
 int hotk_linear_act(const hotk_linear_args* args, void* workspace, size_t ws_bytes, void* stream);
-/* v = in [R, C] times the slope that `save` holds (HOTK_ACT_NONE: times one); out (NULL: none) [R, ld_out], with zeros from C on;
+/* v = in [R, C] times the slope that `save` holds (HOTK_ACT_NONE: times one); out (NULL: none) [R, ld_out], with zeros from C on,
+ * out_lo (NULL: none) of the same layout: what the rounding of out left;
  * partial (NULL: none) [n][C], n = hotk_linear_dz_partials(R): column sums of v in 32 bits, for hotk_sum_partials; total (NULL:
  * none) [C]: the sums themselves, rounded to the type, instead of partial where n is 1 */
 int hotk_linear_dz_partials(int64_t R, int64_t* n_partials);
-int hotk_linear_dz(const void* in, int64_t ld_in, const void* save, int act, void* out, int64_t ld_out, float* partial,
-                   void* total, int64_t R, int64_t C, int type, void* stream);
+int hotk_linear_dz(const void* in, int64_t ld_in, const void* save, int act, void* out, void* out_lo, int64_t ld_out,
+                   float* partial, void* total, int64_t R, int64_t C, int type, void* stream);
 /* rows of `bytes` bytes, ld_in bytes apart, copied to rows ld_out bytes apart (a multiple of 16, out 16-byte aligned) with zeros
  * behind them */
 int hotk_pad_rows(const void* in, int64_t ld_in, void* out, int64_t ld_out, int64_t R, int64_t bytes, void* stream);

@@ -51,7 +51,7 @@ def test_norm_entries_refuse():
 
 def _args(**kw):
     a = dict(M=4, N=8, K=32, x=4096, ld_x=32, w=4096, ld_w=32, bias=0, res=0, ld_res=0, y=4096, ld_y=8, save=0, x_scale=0,
-             w_scale=0, type=1, out_type=1, act=0, flags=0)
+             w_scale=0, type=1, out_type=1, act=0, flags=0, x_lo=0)
     a.update(kw)
     return _lib.LinearArgs(**a)
 
@@ -65,7 +65,8 @@ def _args(**kw):
     ('scales without 8 bits', dict(x_scale=4096, w_scale=4096), EINVAL), ('one scale', dict(type=3, x_scale=4096), EINVAL),
     ('slope of 8 bits', dict(type=3, x_scale=4096, w_scale=4096, save=4096), EINVAL),
     ('half a piece', dict(M=400, K=28, ld_x=28, ld_w=28), EUNSUPPORTED), ('ends inside a piece', dict(M=400, K=28), EUNSUPPORTED), ('x down alone', dict(flags=1, ld_x=8), EUNSUPPORTED),
-    ('unknown flag', dict(flags=8), EINVAL), ('8 bits down', dict(type=3, x_scale=4096, w_scale=4096, flags=2, ld_w=32), EUNSUPPORTED),
+    ('unknown flag', dict(flags=8), EINVAL), ('second part between pieces', dict(flags=2, ld_w=8, x_lo=4098), EUNSUPPORTED),
+    ('second part of 8 bits', dict(type=3, x_scale=4096, w_scale=4096, x_lo=4096), EUNSUPPORTED), ('8 bits down', dict(type=3, x_scale=4096, w_scale=4096, flags=2, ld_w=32), EUNSUPPORTED),
     ('w columns in no whole pieces', dict(flags=2, N=5, ld_w=5, ld_y=5), EUNSUPPORTED), ('row stride', dict(M=400, ld_x=36), EUNSUPPORTED), ('w row stride', dict(M=400, ld_w=36), EUNSUPPORTED),
     ('x between pieces', dict(M=400, x=4098), EUNSUPPORTED), ('w between pieces', dict(M=400, w=4104), EUNSUPPORTED),
     ('x between elements', dict(x=4097), EINVAL), ('w between elements', dict(w=4097), EINVAL),
@@ -89,12 +90,13 @@ def test_product_entry_empty_and_workspace():
 
 
 def test_backward_entries_refuse():
-    dz = lambda i=SOME, ld=8, save=NULL, act=0, out=SOME, ld_o=8, part=NULL, total=NULL, R=4, C=8, ty=1: L.hotk_linear_dz(
-        i, ld, save, act, out, ld_o, part, total, R, C, ty, NULL)
+    dz = lambda i=SOME, ld=8, save=NULL, act=0, out=SOME, lo=NULL, ld_o=8, part=NULL, total=NULL, R=4, C=8, ty=1: L.hotk_linear_dz(
+        i, ld, save, act, out, lo, ld_o, part, total, R, C, ty, NULL)
     assert dz(R=0) == 0
     assert dz(i=NULL) == EINVAL and dz(ld=7) == EINVAL and dz(ld_o=7) == EINVAL and dz(out=NULL) == EINVAL and dz(C=0, ld=0, ld_o=0) == EINVAL
     assert dz(act=3) == EINVAL and dz(act=6, save=SOME) == EINVAL and dz(i=ctypes.c_void_p(4097)) == EINVAL
     assert dz(total=SOME, R=2000) == EINVAL and dz(total=SOME, part=SOME) == EINVAL          # a total of one block only
+    assert dz(out=NULL, lo=SOME, part=SOME) == EINVAL                                        # the rest of nothing
     assert dz(ty=5) == EUNSUPPORTED and dz(ty=3) == EUNSUPPORTED
     n = ctypes.c_int64()
     for R in (0, 1, 16, 17, 8191, 8193, 10 ** 7):

@@ -453,6 +453,33 @@ def test_product_gradients(M, N, K, dt):
             check_gradients(x, w, b, r, act, dy, got, dt)
 
 
+@pytest.mark.parametrize('dt', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('M,N,K', [(50, 200, 130), (700, 24, 64), (2000, 130, 72), (64, 3000, 40)])
+def test_small_gradients_carry_no_rounding_but_their_own(M, N, K, dt):
+    """where the products are short dz enters them in two parts: what is left is the result's rounding (0.58 u as a whole at most,
+    uniform in half a step), where one more rounding would bring 0.8"""
+    from hot_amd import ops
+    x, w, b, _ = linear_case(M, N, K, dt, True, False, seed=155)
+    dy = rnd(156, M, N, dt=dt)
+    z, _ = z_bounds(x, w, b)
+    dz = dy.double() * slope64(z, 'gelu')
+    x.requires_grad_(True), w.requires_grad_(True)
+    dx, dw = torch.autograd.grad(ops.linear_act(x, w, b, act='gelu'), (x, w), dy)
+    for what, got, want in (('dx', dx, dz @ w.detach().double()), ('dw', dw, dz.t() @ x.detach().double())):
+        assert float((got.double() - want).norm() / want.norm()) <= 0.62 * half_step(dt), what
+
+
+def test_infinite_gradients_stay_infinite():
+    """a gradient beyond the type's range is infinite in dz; what its rounding left is nothing, not a NaN"""
+    from hot_amd import ops
+    for dt in (torch.bfloat16, torch.float16):
+        x, w = torch.ones(70, 8, dtype=dt, device=DEV, requires_grad=True), torch.ones(16, 8, dtype=dt, device=DEV)
+        dy = torch.ones(70, 16, dtype=dt, device=DEV)
+        dy[3, 5] = float('inf')
+        dx, = torch.autograd.grad(ops.linear_act(x, w, act='silu'), x, dy)
+        assert (dx[3] == float('inf')).all() and dx[4].isfinite().all()
+
+
 @pytest.mark.parametrize('only', ['x', 'w', 'b', 'r'])
 def test_product_one_gradient_at_a_time(only):
     from hot_amd import ops
