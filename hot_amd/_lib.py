@@ -129,7 +129,7 @@ _SIGNATURES.update({
     'hotk_rmsnorm_quant': [_P, _L, _P, _L, _P, _P, _U, _F, _P, _P, _P, _L, _L, _I, _P],
     'hotk_quantize_rows': [_P, _L, _P, _P, _L, _L, _I, _P],
     'hotk_rmsnorm_partials': [_L, _L, _I, ctypes.POINTER(_L)],
-    'hotk_rmsnorm_bwd': [_P, _L, _P, _L, _P, _L, _P, _P, _P, _U, _P, _P, _L, _L, _I, _P],
+    'hotk_rmsnorm_bwd': [_P, _L, _P, _L, _P, _L, _P, _P, _P, _U, _P, _P, _P, _L, _L, _I, _P],
     'hotk_sum_partials': [_P, _L, _L, _P, _I, _P],
     'hotk_linear_workspace_bytes': [ctypes.POINTER(LinearArgs), ctypes.POINTER(_S)],
     'hotk_linear_act': [ctypes.POINTER(LinearArgs), _P, _S, _P],

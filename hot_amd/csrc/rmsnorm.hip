@@ -207,26 +207,50 @@ struct RnBwd {
   const float* rstd;
   const uint8_t* kind;
   unsigned keep;
-  T* dx;
+  T *dx, *dw;
   float* partial;
   int64_t R;
   int D;
+  unsigned row_blocks;     // the workgroups behind these write dw (few rows), 0: there are none
 };
+
+// dw of few rows: a workgroup takes four pieces of columns, its row lanes every (THREADS / 4)th row each; LDS joins them by halves
+template <class T, int THREADS, bool SMALL>
+__device__ __forceinline__ void rn_columns(const RnBwd<T>& a, typename Elem<T>::fvec* sums) {
+  using FV = typename Elem<T>::fvec;
+  constexpr int LANES = THREADS / 4;
+  const Piece<T, SMALL> p((blockIdx.x - a.row_blocks) * 4 + (threadIdx.x & 3), a.D);
+  FV s = 0.f;
+  for (int64_t row = threadIdx.x >> 2; row < a.R; row += LANES) {
+    if (a.kind && !hotk_keep(a.keep, a.kind[row])) continue;
+    s += p.load(a.dy + row * a.ld_dy, a.D) * (p.load(a.h + row * a.ld_h, a.D) * a.rstd[row]);
+  }
+  sums[threadIdx.x] = s;
+  for (int half = LANES / 2; half >= 1; half >>= 1) {
+    __syncthreads();
+    if ((int)(threadIdx.x >> 2) < half) sums[threadIdx.x] += sums[threadIdx.x + 4 * half];
+  }
+  if (threadIdx.x < 4) p.store(a.dw, a.D, sums[threadIdx.x]);
+}
 
 template <class T, int NV, int LPR, bool SMALL>
 __global__ __launch_bounds__(LPR > 64 ? LPR : 256) void k_rmsnorm_bwd(const RnBwd<T> a) {
   using E = Elem<T>;
   using FV = typename E::fvec;
   constexpr int VEC = E::VEC, GROUPS = LPR > 64 ? 1 : 256 / LPR;
+  constexpr int THREADS = LPR > 64 ? LPR : 256;
+  constexpr bool LATE = NV * VEC >= 32;      // the widest rows: dh is read where it is added, so that what a lane holds stays in registers
   __shared__ float box[2][16];
-  __shared__ FV fold[GROUPS > 1 ? 4 : 1][64];
+  __shared__ FV fold[THREADS];
+  if (a.row_blocks && blockIdx.x >= a.row_blocks) return rn_columns<T, THREADS, SMALL>(a, fold);
+  const unsigned blocks = a.row_blocks ? a.row_blocks : gridDim.x;
   int slot = 0;
   const int t = threadIdx.x % LPR, D = a.D;
   const float inv_d = 1.f / (float)D;
   FV dw[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) dw[i] = 0.f;
-  for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LPR; row < a.R; row += (int64_t)gridDim.x * GROUPS) {
+  for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LPR; row < a.R; row += (int64_t)blocks * GROUPS) {
     if (a.kind && !hotk_keep(a.keep, a.kind[row])) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) Piece<T, SMALL>(t + LPR * i, D).store(a.dx + row * D, D, (FV)0.f);
@@ -240,7 +264,7 @@ __global__ __launch_bounds__(LPR > 64 ? LPR : 256) void k_rmsnorm_bwd(const RnBw
       const Piece<T, SMALL> p(t + LPR * i, D);
       g[i] = p.load(a.dy + row * a.ld_dy, D);
       u[i] = p.load(a.h + row * a.ld_h, D);
-      o[i] = a.dh ? p.load(a.dh + row * a.ld_dh, D) : (FV)0.f;
+      if (!LATE) o[i] = a.dh ? p.load(a.dh + row * a.ld_dh, D) : (FV)0.f;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -255,9 +279,11 @@ __global__ __launch_bounds__(LPR > 64 ? LPR : 256) void k_rmsnorm_bwd(const RnBw
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const Piece<T, SMALL> p(t + LPR * i, D);
+      if (LATE) o[i] = a.dh ? p.load(a.dh + row * a.ld_dh, D) : (FV)0.f;
       p.store(a.dx + row * D, D, o[i] + rstd * (g[i] - u[i] * m));
     }
   }
+  if (!a.partial) return;      // few rows: the workgroups behind these write dw, or nobody wants it
   // one partial row of dw per workgroup: rows side by side in a wave are added across lanes, the waves in order through LDS
   float* out = a.partial + (int64_t)blockIdx.x * D;
 #pragma unroll
@@ -270,11 +296,11 @@ __global__ __launch_bounds__(LPR > 64 ? LPR : 256) void k_rmsnorm_bwd(const RnBw
 #pragma unroll
         for (int d = 32; d >= LPR; d >>= 1) o[k] += __shfl_xor(o[k], d, 64);
       __syncthreads();
-      fold[threadIdx.x >> 6][threadIdx.x & 63] = o;
+      fold[threadIdx.x] = o;
       __syncthreads();
       if (threadIdx.x >= LPR) continue;
 #pragma unroll
-      for (int w = 1; w < 4; ++w) o += fold[w][t];
+      for (int w = 1; w < 4; ++w) o += fold[64 * w + t];
     }
 #pragma unroll
     for (int k = 0; k < VEC; ++k)
@@ -350,14 +376,26 @@ int rn_launch_fwd(const RnFwd<T>& a, hipStream_t st) {
   return hotk_launch_status();
 }
 
+// few rows: dw is written by workgroups of the same launch, which read dy and h once more.  Measured at 1 024 rows against a
+// launch for the partial sums: fp32 of 1 024 columns 8.2 and 10.2 us, 2 048 10.8 and 10.5, 4 096 19.7 and 16.6; bf16 of 2 048 7.3 and 16.3,
+// 4 096 11.0 and 17.2.  A workgroup reads its columns of all rows, which bounds the rows whatever their size.
+bool rn_few(int64_t R, int64_t D, int bytes) { return R <= 1024 && R * D * bytes <= 8 << 20; }
 // workgroups of the backward pass, each with one partial row of dw: enough to fill the chip, few enough that the partial sums
-// stay a few percent of the traffic
-unsigned rn_bwd_grid(int64_t R, int lpr) { return rn_grid(R, rn_rows_per_group(lpr), lpr > 256 ? 512 : 1024); }
+// stay a few percent of the traffic.  Rows of 16 waves: as many as fit at once (16 384 columns of bf16, 1 025 rows: 35 us; 512 of
+// them 50); rows of 4 waves, few of them: 1 025 x 2 048 bf16 11.9 us with 512 and 16.3 with 1 024, 8 192 x 2 048 30.3 and 28.8.
+unsigned rn_bwd_grid(int64_t R, int lpr) {
+  return rn_grid(R, rn_rows_per_group(lpr), lpr > 512 ? 256 : lpr > 256 || (lpr > 64 && R < 8192) ? 512 : 1024);
+}
 
 template <class T>
-int rn_launch_bwd(const RnBwd<T>& a, hipStream_t st) {
+int rn_launch_bwd(RnBwd<T> a, hipStream_t st) {
   const RnShape sh = rn_shape(a.D, Elem<T>::VEC, false);
-  const dim3 grid(rn_bwd_grid(a.R, sh.lpr)), block(sh.lpr > 64 ? sh.lpr : 256);
+  unsigned blocks = rn_bwd_grid(a.R, sh.lpr);
+  if (a.dw) {
+    a.row_blocks = blocks;
+    blocks += (unsigned)((a.D + 4 * Elem<T>::VEC - 1) / (4 * Elem<T>::VEC));
+  }
+  const dim3 grid(blocks), block(sh.lpr > 64 ? sh.lpr : 256);
 #define RN_B(LPR, NV, SMALL) hipLaunchKernelGGL((k_rmsnorm_bwd<T, NV, LPR, SMALL>), grid, block, 0, st, a)
   switch (sh.lpr * 16 + sh.nv) {
     case 8 * 16: RN_B(8, 1, true); break;
@@ -437,23 +475,24 @@ extern "C" int hotk_quantize_rows(const void* x, int64_t ld_x, uint8_t* q, float
 extern "C" int hotk_rmsnorm_partials(int64_t R, int64_t D, int type, int64_t* n_partials) {
   HOTK_CHECK_ARG(n_partials && R >= 0);
   if (!hotk_rmsnorm_supported(D, type)) return HOTK_EUNSUPPORTED;
-  *n_partials = (int64_t)rn_bwd_grid(R, rn_shape(D, 16 / ffn_bytes(type), false).lpr);
+  *n_partials = rn_few(R, D, ffn_bytes(type)) ? 0 : (int64_t)rn_bwd_grid(R, rn_shape(D, 16 / ffn_bytes(type), false).lpr);
   return HOTK_OK;
 }
 
 extern "C" int hotk_rmsnorm_bwd(const void* dy, int64_t ld_dy, const void* dh, int64_t ld_dh, const void* h, int64_t ld_h,
                                 const float* rstd, const void* w, const uint8_t* kind, unsigned keep, void* dx, float* partial,
-                                int64_t R, int64_t D, int type, void* stream) {
+                                void* dw, int64_t R, int64_t D, int type, void* stream) {
   HOTK_CHECK_ARG(R >= 0);
   if (!hotk_rmsnorm_supported(D, type)) return HOTK_EUNSUPPORTED;
-  HOTK_CHECK_ARG(partial);
+  HOTK_CHECK_ARG(rn_few(R, D, ffn_bytes(type)) ? !partial : partial && !dw);
+  HOTK_CHECK_ARG(!dw || ffn_elem_aligned(dw, type));
   HOTK_CHECK_ARG(R == 0 || (rn_rows_ok(dy, ld_dy, D, type) && rn_rows_ok(h, ld_h, D, type) && rstd && rn_rows_ok(dx, D, D, type)));
   HOTK_CHECK_ARG(rn_rows_ok(w, D, D, type) && (!dh || rn_rows_ok(dh, ld_dh, D, type)));
   int rc = HOTK_OK;
   ffn_dispatch(type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
-    const RnBwd<T> a{(const T*)dy, (const T*)dh, (const T*)h, (const T*)w, ld_dy, ld_dh, ld_h, rstd, kind, keep, (T*)dx, partial,
-                     R, (int)D};
+    const RnBwd<T> a{(const T*)dy, (const T*)dh, (const T*)h, (const T*)w, ld_dy, ld_dh, ld_h, rstd, kind, keep, (T*)dx, (T*)dw,
+                     partial, R, (int)D, 0};
     rc = rn_launch_bwd<T>(a, (hipStream_t)stream);
   });
   return rc;

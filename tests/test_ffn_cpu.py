@@ -41,12 +41,13 @@ def test_norm_entries_refuse():
     assert L.hotk_quantize_rows(SOME, 8, NULL, SOME, 2, 8, 0, NULL) == EINVAL
     assert L.hotk_quantize_rows(NULL, 8, NULL, NULL, 0, 8, 0, NULL) == 0
     assert L.hotk_rmsnorm_quant(SOME, 8, NULL, 0, SOME, NULL, 6, 1e-6, SOME, NULL, NULL, 2, 8, 0, NULL) == EINVAL
-    assert L.hotk_rmsnorm_bwd(SOME, 8, NULL, 0, SOME, 8, NULL, SOME, NULL, 6, SOME, SOME, 2, 8, 0, NULL) == EINVAL
-    assert L.hotk_rmsnorm_bwd(SOME, 8, NULL, 0, SOME, 8, SOME, SOME, NULL, 6, SOME, NULL, 2, 8, 0, NULL) == EINVAL
+    bwd = lambda rstd=SOME, part=NULL, dw=SOME, R=2: L.hotk_rmsnorm_bwd(SOME, 8, NULL, 0, SOME, 8, rstd, SOME, NULL, 6, SOME, part, dw, R, 8, 0, NULL)
+    assert bwd(rstd=NULL) == EINVAL and bwd(part=SOME) == EINVAL                      # few rows: no partial sums
+    assert bwd(R=5000) == EINVAL and bwd(R=5000, part=SOME) == EINVAL                 # many: those, and no dw
     assert L.hotk_sum_partials(NULL, 3, 4, SOME, 0, NULL) == EINVAL and L.hotk_sum_partials(NULL, 0, 0, NULL, 0, NULL) == 0
     n = ctypes.c_int64()
-    for R, D, ty in ((0, 8, 0), (1, 8, 1), (100000, 8, 2), (100000, 32768, 0)):
-        assert L.hotk_rmsnorm_partials(R, D, ty, ctypes.byref(n)) == 0 and 1 <= n.value <= max(1, R)
+    for R, D, ty in ((0, 8, 0), (1, 8, 1), (1024, 8, 1), (1025, 8, 1), (100000, 8, 2), (100000, 32768, 0)):
+        assert L.hotk_rmsnorm_partials(R, D, ty, ctypes.byref(n)) == 0 and min(1, R // 1025) <= n.value <= R // 1025 * R
 
 
 def _args(**kw):

@@ -67,7 +67,7 @@ def norm_case(R, D, dt, residual, mask, seed=0):
 
 
 NORM_SIZES = [(1, 1), (3, 3), (5, 7), (2, 8), (7, 9), (4, 15), (65, 33), (9, 255), (8, 256), (6, 257), (5, 1000), (3, 1001), (17, 2048),
-              (3, 2049), (2, 4100), (3, 8191)]
+              (3, 2049), (2, 4100), (3, 8191), (1024, 40), (1025, 40), (3000, 7), (2500, 300)]
 
 
 @pytest.mark.parametrize('dt', TYPES)
@@ -749,3 +749,18 @@ def test_refusals():
             raise AssertionError(f'call {i} was taken')
     with torch.no_grad():
         ops.quantize_rows(x.clone().requires_grad_(True))
+
+
+@pytest.mark.parametrize('R,D', [(1, 5), (5, 24), (1024, 40), (1025, 40), (6, 2049)])
+def test_norm_gradients_of_some_inputs(R, D):
+    """x, the weight or the residual alone: each gradient is the one that all together get"""
+    from hot_amd import ops
+    leaves = [rnd(401, R, D), rnd(402, D), rnd(403, R, D)]
+    dy, dh = rnd(404, R, D), rnd(405, R, D)
+    def grads(which):
+        x, w, r = [l.clone().requires_grad_(i in which) for i, l in enumerate(leaves)]
+        return dict(zip(which, torch.autograd.grad(ops.rms_norm(x, w, r), [(x, w, r)[i] for i in which], (dy, dh))))
+    both = grads((0, 1, 2))
+    for which in ((0,), (1,), (2,), (0, 1), (1, 2)):
+        for i, g in grads(which).items():
+            assert torch.equal(g, both[i])

@@ -184,7 +184,7 @@ def test_first_order_only():
 
 def test_launches_are_timed_like_the_framework_s_others():
     from hot_amd import _lib, ops
-    x, w = torch.randn(70, 16, device=DEV, requires_grad=True), torch.randn(24, 16, device=DEV, requires_grad=True)
+    x, w = torch.randn(1100, 16, device=DEV, requires_grad=True), torch.randn(24, 16, device=DEV, requires_grad=True)
     _lib.timing_begin(None)
     ops.linear_act(ops.rms_norm(x, w[0]), w, act='gelu').sum().backward()
     seen = _lib.timing_end()
