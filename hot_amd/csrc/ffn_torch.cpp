@@ -115,6 +115,12 @@ int type_of(at::ScalarType t) {
   }
 }
 
+// the values are what the memory holds
+void check_memory(const Tensor& t, const char* what) {
+  if (t.layout() != at::kStrided) refuse(what, ": a strided tensor is expected");
+  if (t.is_neg() || t._is_zerotensor()) refuse(what, " is a view that negates (or stands for zeros without memory): call resolve_neg() or clone() first");
+}
+
 void check_input(const Tensor& x, const char* what, bool eight = false) {
   if (!x.defined()) refuse(what, ": a tensor is expected");
   if (!x.is_cuda())
@@ -122,7 +128,7 @@ void check_input(const Tensor& x, const char* what, bool eight = false) {
   const int ty = type_of(x.scalar_type());
   if (eight ? ty != HOTK_E4M3 : (ty < 0 || ty == HOTK_E4M3))
     refuse(what, ": ", eight ? "float8_e4m3fn" : "fp32, bf16 or fp16", " expected, got ", x.scalar_type());
-  if (x.layout() != at::kStrided) refuse(what, ": a strided tensor is expected");
+  check_memory(x, what);
   if (x.dim() < 1 || x.size(-1) == 0) refuse(what, ": [..., width] with width >= 1 expected, got shape ", x.sizes());
 }
 
@@ -131,7 +137,7 @@ void check_with(const Tensor& ref, const Tensor& t, const char* what, at::IntArr
   if (!t.defined()) refuse(what, ": a tensor is expected");
   if (t.device() != ref.device()) refuse(what, " is on ", t.device(), ", the input on ", ref.device());
   if (t.scalar_type() != type) refuse(what, ": ", type, " expected, got ", t.scalar_type());
-  if (t.layout() != at::kStrided) refuse(what, ": a strided tensor is expected");
+  check_memory(t, what);
   if (t.sizes() != shape) refuse(what, ": shape ", shape, " expected, got ", t.sizes());
 }
 
@@ -143,7 +149,9 @@ struct Rows {
   const void* p() const { return t.defined() ? t.const_data_ptr() : nullptr; }
 };
 
-Rows rows(const Tensor& x) {
+Rows rows(const Tensor& given) {
+  // (a gradient may be such a view; inputs were checked)
+  const Tensor x = given.is_neg() || given._is_zerotensor() ? given.clone() : given;
   const int64_t C = x.size(-1), n = x.numel() / C;
   if (n == 0) return {x, C, 0};
   if (x.stride(-1) == 1 || C == 1) {

@@ -764,3 +764,42 @@ def test_norm_gradients_of_some_inputs(R, D):
     for which in ((0,), (1,), (2,), (0, 1), (1, 2)):
         for i, g in grads(which).items():
             assert torch.equal(g, both[i])
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('R,D', [(2, 12001), (90, 32767), (130, 20000)])
+def test_wide_rows_with_all_gradients(R, D, dt):
+    """the widest rows (dh read late), weight gradients of few rows as one launch and as partial sums"""
+    from hot_amd import ops
+    x, w, r, _ = norm_case(R, D, dt, True, False, seed=410)
+    for t in (x, w, r):
+        t.requires_grad_(True)
+    dy, dh = rnd(414, R, D, dt=dt), rnd(415, R, D, dt=dt)
+    dx, dw, dr = torch.autograd.grad(ops.rms_norm(x, w, r), (x, w, r), (dy, dh))
+    h64, inv, _ = norm64(x.detach(), w.detach(), r.detach(), 1e-6, None, dt)
+    g, unit = dy.double() * w.detach().double(), h64 * inv
+    want = inv * (g - unit * (g * unit).mean(-1, keepdim=True)) + dh.double()
+    size = inv * (g.abs() + unit.abs() * (g * unit).abs().mean(-1, keepdim=True)) + dh.double().abs()
+    hold('dx', dx, want, half_step(dt) * want.abs() + 3 * CHAIN * E * size + floor_of(dt))
+    assert torch.equal(dx, dr)
+    want = (dy.double() * unit).sum(0)
+    hold('dw', dw, want, half_step(dt) * want.abs() + (CHAIN + R) * E * (dy.double() * unit).abs().sum(0) + floor_of(dt))
+
+
+def test_views_that_negate():
+    """a lazily negated view's memory holds other values: inputs are refused, a gradient is resolved"""
+    from hot_amd import ops
+    from hot_amd._lib import HotkError
+    z = torch.complex(rnd(420, 6, 16), rnd(421, 6, 16))
+    neg = z.conj().imag
+    assert neg.is_neg()
+    w = rnd(422, 16)
+    for call in (lambda: ops.rms_norm(neg, w), lambda: ops.rms_norm(z.imag, w, neg), lambda: ops.rms_norm(z.imag, neg[0]), lambda: ops.quantize_rows(neg),
+                 lambda: ops.linear_act(neg, neg.resolve_neg()), lambda: ops.linear_act(neg.resolve_neg(), neg)):
+        with pytest.raises(HotkError, match='resolve_neg'):
+            call()
+    x = rnd(423, 6, 16).requires_grad_(True)
+    for f in (lambda: ops.rms_norm(x, w), lambda: ops.linear_act(x, neg.resolve_neg(), act='gelu')):
+        y = f()
+        dy = neg if y.shape == neg.shape else neg[:, :6]
+        assert torch.equal(torch.autograd.grad(y, x, dy)[0], torch.autograd.grad(f(), x, dy.resolve_neg())[0])
