@@ -803,3 +803,20 @@ def test_views_that_negate():
         y = f()
         dy = neg if y.shape == neg.shape else neg[:, :6]
         assert torch.equal(torch.autograd.grad(y, x, dy)[0], torch.autograd.grad(f(), x, dy.resolve_neg())[0])
+
+
+@pytest.mark.parametrize('M,K,N', [(1, 742, 36), (70, 37, 24), (65, 64, 40)])
+def test_kept_tensors_that_left_the_device(M, K, N):
+    """what the forward pass keeps comes back from the host with strides of its own"""
+    from hot_amd import ops
+    leaves = [rnd(430, M, K + 9)[:, 3:K + 3], rnd(431, K, N).t(), rnd(432, N), rnd(433, M, N)]
+    dy = rnd(434, M, N)
+    def grads():
+        x, w, b, r = [l.detach().requires_grad_(True) for l in leaves]
+        y = ops.linear_act(x, w, b, act='silu', residual=r)
+        z = ops.rms_norm(x, w[0])
+        return torch.autograd.grad((y, z), (x, w, b, r), (dy, dy[:, :1].expand(M, K)))
+    with torch.autograd.graph.save_on_cpu():
+        got = grads()
+    want = grads()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
