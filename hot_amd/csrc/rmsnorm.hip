@@ -18,6 +18,8 @@
 // Measured (a large copy reads and writes 5.0 TB/s here): 16 384 x 4 096 bf16 with a residual 88 us forward (6.1 TB/s of x, r, h, y)
 // and 103 + 5 backward (5.2 TB/s); 8 192 x 2 048 bf16 to 8 bits 25 us (4.7 TB/s); rows of 8 192 x 4 096 bf16 to 8 bits 18 us (5.5);
 // one row of 4 096: 2.5 us, a launch.
+#include <algorithm>
+
 #include "ffn.h"
 
 namespace {
@@ -211,7 +213,6 @@ struct RnBwd {
   float* partial;
   int64_t R;
   int D;
-  unsigned row_blocks;     // the workgroups behind these write dw (few rows), 0: there are none
 };
 
 // dw of few rows: a workgroup takes four pieces of columns, its row lanes every (THREADS / 4)th row each; LDS joins them by halves
@@ -219,7 +220,8 @@ template <class T, int THREADS, bool SMALL>
 __device__ __forceinline__ void rn_columns(const RnBwd<T>& a, typename Elem<T>::fvec* sums) {
   using FV = typename Elem<T>::fvec;
   constexpr int LANES = THREADS / 4;
-  const Piece<T, SMALL> p((blockIdx.x - a.row_blocks) * 4 + (threadIdx.x & 3), a.D);
+  if ((int64_t)blockIdx.x * 4 * Elem<T>::VEC >= a.D) return;
+  const Piece<T, SMALL> p(blockIdx.x * 4 + (threadIdx.x & 3), a.D);
   FV s = 0.f;
   for (int64_t row = threadIdx.x >> 2; row < a.R; row += LANES) {
     if (a.kind && !hotk_keep(a.keep, a.kind[row])) continue;
@@ -233,7 +235,8 @@ __device__ __forceinline__ void rn_columns(const RnBwd<T>& a, typename Elem<T>::
   if (threadIdx.x < 4) p.store(a.dw, a.D, sums[threadIdx.x]);
 }
 
-template <class T, int NV, int LPR, bool SMALL>
+// FEW: few rows, dw wanted.  (An instance of its own: with the branch in all of them 16 384 x 4 096 bf16 took 107 us instead of 98.)
+template <class T, int NV, int LPR, bool SMALL, bool FEW>
 __global__ __launch_bounds__(LPR > 64 ? LPR : 256) void k_rmsnorm_bwd(const RnBwd<T> a) {
   using E = Elem<T>;
   using FV = typename E::fvec;
@@ -242,15 +245,14 @@ __global__ __launch_bounds__(LPR > 64 ? LPR : 256) void k_rmsnorm_bwd(const RnBw
   constexpr bool LATE = NV * VEC >= 32;      // the widest rows: dh is read where it is added, so that what a lane holds stays in registers
   __shared__ float box[2][16];
   __shared__ FV fold[THREADS];
-  if (a.row_blocks && blockIdx.x >= a.row_blocks) return rn_columns<T, THREADS, SMALL>(a, fold);
-  const unsigned blocks = a.row_blocks ? a.row_blocks : gridDim.x;
+  if (FEW && blockIdx.y) return rn_columns<T, THREADS, SMALL>(a, fold);
   int slot = 0;
   const int t = threadIdx.x % LPR, D = a.D;
   const float inv_d = 1.f / (float)D;
   FV dw[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) dw[i] = 0.f;
-  for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LPR; row < a.R; row += (int64_t)blocks * GROUPS) {
+  for (int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LPR; row < a.R; row += (int64_t)gridDim.x * GROUPS) {
     if (a.kind && !hotk_keep(a.keep, a.kind[row])) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) Piece<T, SMALL>(t + LPR * i, D).store(a.dx + row * D, D, (FV)0.f);
@@ -283,7 +285,7 @@ __global__ __launch_bounds__(LPR > 64 ? LPR : 256) void k_rmsnorm_bwd(const RnBw
       p.store(a.dx + row * D, D, o[i] + rstd * (g[i] - u[i] * m));
     }
   }
-  if (!a.partial) return;      // few rows: the workgroups behind these write dw, or nobody wants it
+  if (FEW || !a.partial) return;      // few rows: the grid's second line writes dw, or nobody wants it
   // one partial row of dw per workgroup: rows side by side in a wave are added across lanes, the waves in order through LDS
   float* out = a.partial + (int64_t)blockIdx.x * D;
 #pragma unroll
@@ -376,9 +378,9 @@ int rn_launch_fwd(const RnFwd<T>& a, hipStream_t st) {
   return hotk_launch_status();
 }
 
-// few rows: dw is written by workgroups of the same launch, which read dy and h once more.  Measured at 1 024 rows against a
-// launch for the partial sums: fp32 of 1 024 columns 8.2 and 10.2 us, 2 048 10.8 and 10.5, 4 096 19.7 and 16.6; bf16 of 2 048 7.3 and 16.3,
-// 4 096 11.0 and 17.2.  A workgroup reads its columns of all rows, which bounds the rows whatever their size.
+// few rows: dw is written by a second line of workgroups of the same launch, which read dy and h once more.  Measured at 1 024 rows
+// against a launch for the partial sums: fp32 of 1 024 columns 5.9 and 10.2 us, 2 048 10.8 and 10.5, 4 096 19.7 and 16.6; bf16 of 2 048 6.8
+// and 11.9, 4 096 10.9 and 17.1.  A workgroup reads its columns of all rows, which bounds the rows whatever their size.
 bool rn_few(int64_t R, int64_t D, int bytes) { return R <= 1024 && R * D * bytes <= 8 << 20; }
 // workgroups of the backward pass, each with one partial row of dw: enough to fill the chip, few enough that the partial sums
 // stay a few percent of the traffic.  Rows of 16 waves: as many as fit at once (16 384 columns of bf16, 1 025 rows: 35 us; 512 of
@@ -388,15 +390,14 @@ unsigned rn_bwd_grid(int64_t R, int lpr) {
 }
 
 template <class T>
-int rn_launch_bwd(RnBwd<T> a, hipStream_t st) {
+int rn_launch_bwd(const RnBwd<T>& a, hipStream_t st) {
   const RnShape sh = rn_shape(a.D, Elem<T>::VEC, false);
-  unsigned blocks = rn_bwd_grid(a.R, sh.lpr);
-  if (a.dw) {
-    a.row_blocks = blocks;
-    blocks += (unsigned)((a.D + 4 * Elem<T>::VEC - 1) / (4 * Elem<T>::VEC));
-  }
-  const dim3 grid(blocks), block(sh.lpr > 64 ? sh.lpr : 256);
-#define RN_B(LPR, NV, SMALL) hipLaunchKernelGGL((k_rmsnorm_bwd<T, NV, LPR, SMALL>), grid, block, 0, st, a)
+  // few rows: a second line of workgroups writes dw
+  const unsigned blocks = rn_bwd_grid(a.R, sh.lpr), columns = (unsigned)((a.D + 4 * Elem<T>::VEC - 1) / (4 * Elem<T>::VEC));
+  const dim3 grid(a.dw ? std::max(blocks, columns) : blocks, a.dw ? 2 : 1), block(sh.lpr > 64 ? sh.lpr : 256);
+#define RN_B(LPR, NV, SMALL)                                                                    \
+  if (a.dw) hipLaunchKernelGGL((k_rmsnorm_bwd<T, NV, LPR, SMALL, true>), grid, block, 0, st, a); \
+  else hipLaunchKernelGGL((k_rmsnorm_bwd<T, NV, LPR, SMALL, false>), grid, block, 0, st, a)
   switch (sh.lpr * 16 + sh.nv) {
     case 8 * 16: RN_B(8, 1, true); break;
     case 8 * 16 + 1: RN_B(8, 1, false); break;
@@ -409,7 +410,7 @@ int rn_launch_bwd(RnBwd<T> a, hipStream_t st) {
     case 512 * 16 + 2: RN_B(512, 2, false); break;
     case 1024 * 16 + 2: RN_B(1024, 2, false); break;
     case 1024 * 16 + 4: RN_B(1024, 4, false); break;
-    default: if constexpr (Elem<T>::VEC == 4) RN_B(1024, 8, false);
+    default: if constexpr (Elem<T>::VEC == 4) { RN_B(1024, 8, false); }
   }
 #undef RN_B
   return hotk_launch_status();
@@ -492,7 +493,7 @@ extern "C" int hotk_rmsnorm_bwd(const void* dy, int64_t ld_dy, const void* dh, i
   ffn_dispatch(type, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     const RnBwd<T> a{(const T*)dy, (const T*)dh, (const T*)h, (const T*)w, ld_dy, ld_dh, ld_h, rstd, kind, keep, (T*)dx, (T*)dw,
-                     partial, R, (int)D, 0};
+                     partial, R, (int)D};
     rc = rn_launch_bwd<T>(a, (hipStream_t)stream);
   });
   return rc;
