@@ -675,19 +675,21 @@ __global__ __launch_bounds__(256) void k_linact_dz(const T* __restrict__ in, int
   const int64_t r1 = (block + 1) * rows < R ? (block + 1) * rows : R;
   const int left = (int)(C - c < E::VEC ? (C > c ? C - c : 0) : E::VEC), room = (int)(ld_out - c < E::VEC ? (ld_out > c ? ld_out - c : 0) : E::VEC);
   FV s = 0.f;
-  if (left > 0 || (out && room > 0)) {
+  // WHOLE: a whole piece on either side, no test between the loads, so that those of several rows are under way together
+  const auto block_rows = [&](auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll 2
     for (int64_t r = block * rows + rl; r < r1; r += rstep) {
       FV v = 0.f;
-      if (left > 0) {
-        v = ffn_load(in + r * ld_in + c, 0, left);
+      if (WHOLE || left > 0) {
+        v = WHOLE ? ffn_load(in + r * ld_in + c, 0, E::VEC) : ffn_load(in + r * ld_in + c, 0, left);
         if (act != HOTK_ACT_NONE) {
           if constexpr (std::is_same<T, float>::value) {
-            la_times_slope(v, ffn_load((const float*)save + r * C + c, 0, left), act);
+            la_times_slope(v, ffn_load((const float*)save + r * C + c, 0, WHOLE ? E::VEC : left), act);
           } else {
             typedef int16_t s16x8u __attribute__((ext_vector_type(8), aligned(2)));
             const int16_t* codes = (const int16_t*)save + r * C + c;
-            if (left == E::VEC) {
+            if (WHOLE) {
               const s16x8u d = *reinterpret_cast<const s16x8u*>(codes);
 #pragma unroll
               for (int k = 0; k < E::VEC; ++k) v[k] *= la_slope(d[k], act);
@@ -700,23 +702,28 @@ __global__ __launch_bounds__(256) void k_linact_dz(const T* __restrict__ in, int
         }
         s += v;
       }
-      if (out && room > 0) {
-        ffn_store(out + r * ld_out + c, 0, room, v);
+      if (out && (WHOLE || room > 0)) {
+        ffn_store(out + r * ld_out + c, 0, WHOLE ? E::VEC : room, v);
         if (out_lo) {
           const FV hi = __builtin_convertvector(__builtin_convertvector(v, typename E::vec), FV);
           FV lo;
 #pragma unroll
           for (int k = 0; k < E::VEC; ++k) lo[k] = hi[k] - hi[k] == 0.f ? v[k] - hi[k] : 0.f;     // (an infinity leaves nothing)
-          ffn_store(out_lo + r * ld_out + c, 0, room, lo);
+          ffn_store(out_lo + r * ld_out + c, 0, WHOLE ? E::VEC : room, lo);
         }
       }
     }
-  }
+  };
+  if (left == E::VEC && (!out || room == E::VEC)) block_rows(std::true_type{});
+  else if (left > 0 || (out && room > 0)) block_rows(std::false_type{});
   if (partial || total) {
     sums[threadIdx.x] = s;
-    __syncthreads();
+    for (int half = rstep / 2; half >= 1; half /= 2) {
+      __syncthreads();
+      if (rl < half) sums[threadIdx.x] += sums[threadIdx.x + (half << cg_log)];
+    }
     if (rl == 0) {
-      for (int i = 1; i < rstep; ++i) s += sums[(i << cg_log) + piece];
+      s = sums[threadIdx.x];
 #pragma unroll
       for (int k = 0; k < E::VEC; ++k)
         if (k < left) {
@@ -944,8 +951,12 @@ extern "C" int hotk_linear_dz(const void* in, int64_t ld_in, const void* save, i
   if (R == 0) return HOTK_OK;
   HOTK_CHECK_ARG(in);
   const int64_t pieces = la_div(out ? ld_out : C, 16 / ffn_bytes(type)), rows = la_dz_rows(R), down = la_div(R, rows);
-  int cg_log = 0;                          // 32 pieces side by side; 4 where one block has many rows
-  while (cg_log < (rows >= 1024 && R > 64 ? 2 : 5) && (1 << cg_log) < pieces) ++cg_log;
+  // 32 pieces side by side (16 384 x 4 096 bf16 76 us; 4 of them 153), 16 where a block has many rows (700 000 x 256: 223 and 292); one
+  // block of up to 1 024 rows has few workgroups and goes by its rows' time: 2 pieces (1 000 x 4 096: 15 us, 4 of them 19, 32 of them
+  // 76), 4 of up to 64 rows (64 x 4 096: 3.7 and 7.4 with 32)
+  const int most = down == 1 ? (R > 64 ? 1 : 2) : rows >= 1024 ? 4 : 5;
+  int cg_log = 0;
+  while (cg_log < most && (1 << cg_log) < pieces) ++cg_log;
   const int64_t across = la_div(pieces, 1 << cg_log);
   if (across * down >= 2 * LA_MAX_GRID || rows > (1 << 30)) return HOTK_ETOOLARGE;
   ffn_dispatch(type, [&](auto* tag) {
