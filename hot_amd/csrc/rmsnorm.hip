@@ -16,7 +16,7 @@
 // element in one lane only, the stores write the same values twice.  Rows shorter than VEC go element by element (SMALL).
 //
 // Measured (a large copy reads and writes 5.0 TB/s here): 16 384 x 4 096 bf16 with a residual 88 us forward (6.1 TB/s of x, r, h, y)
-// and 103 + 5 backward (5.2 TB/s); 8 192 x 2 048 bf16 to 8 bits 25 us (4.7 TB/s); rows of 8 192 x 4 096 bf16 to 8 bits 18 us (5.5);
+// and 98 to 112 + 5 backward (5.5 to 4.8 TB/s); 8 192 x 2 048 bf16 to 8 bits 25 us (4.7 TB/s); rows of 8 192 x 4 096 bf16 to 8 bits 18 us (5.5);
 // one row of 4 096: 2.5 us, a launch.
 #include <algorithm>
 

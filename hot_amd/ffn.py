@@ -65,7 +65,8 @@ def linear_act(x, weight, bias=None, act='none', residual=None):
     'tanh', 'silu'.  Differentiable in x, weight, bias and residual.
 
     Rows that start at 16-byte boundaries and hold whole 16-byte pieces (K a multiple of 8, of 4 in fp32) are read in place;
-    others are copied once with zeros behind them.  Rows of up to 8 MiB, else HotkError."""
+    others are copied once with zeros behind them; up to 64 rows of x, where the kernel for few rows is the faster one, are
+    read at any alignment, and the weight with them.  Rows of up to 8 MiB, else HotkError."""
     try:
         return (_binding or _ext()).linear_act(x, weight, bias, act, residual)
     except TypeError as e:
