@@ -52,22 +52,30 @@ class EncLayer(nn.Module):
 
     def quantize_feed_forward(self):
         """keep the feed-forward weights in 8 bits too, for calls in eval mode without gradients; taken from the weights as they
-        are now: a forward call that finds them changed since raises.  They are not part of the state_dict"""
+        are now: a forward call that finds them changed, moved or replaced since raises (values written through .data are not
+        seen).  They are part of neither the state_dict nor a copy or pickle of the module, which serve the full weights"""
         if self.norm != 'rmsnorm':
             raise HotkError("8-bit feed-forward products need norm='rmsnorm'")
         for name, t in zip(_EIGHT, _stack.quantize_block(self.ffn)):
             self.register_buffer(name, t, persistent=False)
-        self._eight_of = self._versions()
+        self._eight_of = [(w, w.data_ptr(), w._version) for w in self._ffn_weights()]
 
-    def _versions(self):
-        return [self.ffn[i].weight._version for i in (1, 3)]
+    def _ffn_weights(self):
+        return self.ffn[1].weight, self.ffn[3].weight
+
+    def __getstate__(self):
+        state = self.__dict__.copy()
+        if state.pop('_eight_of', None) is not None:
+            state['_buffers'] = type(self._buffers)((k, v) for k, v in self._buffers.items() if k not in _EIGHT)
+            state['_non_persistent_buffers_set'] = self._non_persistent_buffers_set - set(_EIGHT)
+        return state
 
     def forward(self, x, indices=None):
         attended = self.attn(self.ln(x), indices)
         if self.norm == 'rmsnorm':
             eight = None
             if not self.training and not torch.is_grad_enabled() and hasattr(self, _EIGHT[0]):
-                if self._eight_of != self._versions():
+                if not all(w is v and w.data_ptr() == at and w._version == n for w, (v, at, n) in zip(self._ffn_weights(), self._eight_of)):
                     raise HotkError('the feed-forward weights have changed since quantize_feed_forward(): call it again')
                 eight = [getattr(self, name) for name in _EIGHT]
             return _stack.feed_forward(self.ffn, attended, x if self.residual else None, eight)

@@ -109,6 +109,38 @@ def test_uniform_encoder_serves_in_8_bits():
         EncLayer(1, 1, 16, 8, 8, 16, 2, att_cfg='generalized_kernel', feature_map=enc.feature_map).quantize_feed_forward()
 
 
+def test_quantized_encoder_copies_and_replaced_weights():
+    """a copy or a pickle serves the full weights, also after its own have changed; weights replaced as a whole are noticed"""
+    import copy
+    import io
+    from hot_amd._lib import HotkError
+    enc, x, idx = uniform(seed=9)
+    enc.eval()
+    with torch.no_grad():
+        full = enc(x, idx)
+        eight = enc.quantize_feed_forward()(x, idx)
+        assert not torch.equal(eight, full)
+        f = io.BytesIO()
+        torch.save(enc, f)
+        f.seek(0)
+        for other in (copy.deepcopy(enc), torch.load(f, weights_only=False)):
+            assert torch.equal(other(x, idx), full)
+            w = other.layers[1].ffn[1].weight
+            changed = []
+            for _ in range(4):                                       # whatever number its version has
+                w.mul_(1.25)
+                changed.append(other(x, idx))
+            assert not any(torch.equal(c, full) for c in changed)
+            assert not torch.equal(other.quantize_feed_forward()(x, idx), changed[-1])
+        assert torch.equal(enc(x, idx), eight)
+        lin = enc.layers[0].ffn[3]
+        for change in (lambda: setattr(lin, 'weight', torch.nn.Parameter(lin.weight * 2)), lambda: setattr(lin.weight, 'data', lin.weight * 2)):
+            change()
+            with pytest.raises(HotkError):
+                enc(x, idx)
+            enc.quantize_feed_forward()(x, idx)
+
+
 def sparse_batch(seed, sizes=(9, 5, 12)):
     from hot_amd.batch import sparse as bs
     from hot_amd.utils.graphs import ba_edges
