@@ -197,11 +197,14 @@ __device__ __forceinline__ void la_finish(const LaEpi<OT>& e, int64_t m, int64_t
   if (left <= 0) return;
   if (e.xs) {
     const float xs = e.xs[m];
+    const bool large = fabsf(xs) > 1.f;  // then w's scale goes first: nothing overflows on the way that the result holds
 #pragma unroll
     for (int i = 0; i < W; i += 4) {
       const f32x4 s = ffn_load(e.ws + n0, i, left);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) z[i + k] = z[i + k] * xs * s[k];
+      for (int k = 0; k < 4; ++k) z[i + k] *= large ? s[k] : xs;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) z[i + k] *= large ? xs : s[k];
     }
   }
   if (e.bias) {

@@ -820,3 +820,22 @@ def test_kept_tensors_that_left_the_device(M, K, N):
         got = grads()
     want = grads()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('M', [3, 200])
+@pytest.mark.parametrize('dt', [torch.float32, torch.bfloat16])
+def test_scales_far_apart(M, dt):
+    """one operand near the top of the range, the other small: the result is what the product holds, either way round"""
+    from hot_amd import ops
+    K, N = 256, 48
+    x, w = rnd(440, M, K), rnd(441, N, K)
+    for up, down in ((2.0 ** 120, 2.0 ** -110), (2.0 ** -110, 2.0 ** 120)):
+        (xq, sx), (wq, sw) = ops.quantize_rows(x * up), ops.quantize_rows(w * down)
+        got = ops.linear_act_quantized(xq, sx, wq, sw, out_dtype=dt)
+        scale = sx.double()[:, None] * sw.double()
+        want, size = (xq.double() @ wq.double().t()) * scale, (xq.double().abs() @ wq.double().abs().t()) * scale
+        # 16-bit results: the eights' own 2^-10 of the sums (fp32: K additions in 32 bits), two products, one rounding
+        hold('y', got, want, half_step(dt) * want.abs() + ((K + 4) * E if dt == torch.float32 else 2.0 ** -10) * size)
+    sx[0], sw[1] = float('nan'), float('nan')
+    got = ops.linear_act_quantized(xq, sx, wq, sw, out_dtype=dt)
+    assert got[0].isnan().all() and got[:, 1].isnan().all() and got[1:, 2:].isfinite().all()
