@@ -596,13 +596,24 @@ __global__ __launch_bounds__(512) void k_linact_few(const LaTile<OT> g) {
     xrow[b] = g.a + (16 * b + lr < g.M ? 16 * b + lr : g.M - 1) * g.lda;
     acc[b] = 0.f;
   }
-  // rows may start anywhere and end inside a piece: what lies behind the end is not read, and counts as zero
+  // rows may start anywhere and end inside a piece: what lies behind the end counts as zero.  Loads off a word's start are split
+  // by the hardware (64 x 2 101 -> 128 bf16: 29 us): such rows are read by the words that hold them, and shifted (18 us)
+  const bool off_word = E < 4 && (((uintptr_t)g.a | (uintptr_t)g.b | (uint64_t)g.lda | (uint64_t)g.ldb) & 3) != 0;
   auto piece = [&](const char* row, int64_t c) {
-    typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(1)));
+    typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(4)));
     u32x4 v = 0;
     const int64_t at = c * 16;
     if (at + 16 <= bytes) {
-      v = *reinterpret_cast<const u32x4u*>(row + at);
+      if (!off_word) {
+        v = *reinterpret_cast<const u32x4u*>(row + at);
+      } else {
+        const unsigned shift = (unsigned)((uintptr_t)(row + at) & 3);
+        const uint32_t* word = reinterpret_cast<const uint32_t*>(row + at - shift);
+        const u32x4 t = *reinterpret_cast<const u32x4u*>(word);
+        const uint32_t next = word[shift ? 4 : 3];       // (at a word's start there is no fifth)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_alignbyte(i < 3 ? t[i + 1] : next, t[i], shift);
+      }
     } else if (at < bytes) {
 #pragma unroll
       for (int i = 0; i < 16; i += E)
@@ -766,7 +777,7 @@ int64_t la_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct LaShape { int bm, bn, splits; };      // bn 16: k_linact_few, bm / 16 blocks of rows
 struct LaCost { int bm, bn; float sat, lat, end; };
 const LaCost LA_COSTS[] = {{256, 256, 1.58f, 1.58f, 6.f}, {128, 128, 0.42f, 0.69f, 3.f}, {64, 128, 0.26f, 0.39f, 1.2f}, {64, 64, 0.16f, 0.32f, 0.7f}};
-LaShape la_shape(int64_t M, int64_t N, int64_t K, int type, int out_type, int flags, bool whole, int parts) {
+LaShape la_shape(int64_t M, int64_t N, int64_t K, int type, int out_type, int flags, bool whole, bool off_word, int parts) {
   const int64_t ktiles = la_div(K * ffn_bytes(type), 128) * parts;
   const bool wide = type == HOTK_E4M3 && out_type == HOTK_F32;
   const float mfma = type == HOTK_F32 ? 8.f : wide ? 2.f : 1.f;
@@ -775,8 +786,8 @@ LaShape la_shape(int64_t M, int64_t N, int64_t K, int type, int out_type, int fl
   if (M <= 64 && flags == 0 && parts == 1) {     // k_linact_few: 8.6 TB/s in all, 50 GB/s a compute unit, its matrix work beside that
     const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
     const float wgs = (float)la_div(N, 16), bytes = ktiles * 128.f * 16 * (1 + mb);
-    // (rows in no whole pieces: the tiles would need two copies first)
-    least = -(whole ? 0.f : 8.f) + std::max(std::max(wgs * bytes / 8.6e6f, std::ceil(wgs / 256.f) * bytes / 50e3f),
+    // (rows in no whole pieces: the tiles would need two copies first; off a word's start the loads take 1.7 times as long)
+    least = -(whole ? 0.f : 8.f) + std::max((off_word ? 1.7f : 1.f) * std::max(wgs * bytes / 8.6e6f, std::ceil(wgs / 256.f) * bytes / 50e3f),
                      std::ceil(wgs / 256.f) * ktiles * 0.89f * mfma * mb / 256.f);
     best = {16 * mb, 16, 1};
   }
@@ -873,7 +884,11 @@ bool la_whole(const hotk_linear_args& a) {
   return a.ld_x >= la_div(row_x, m) * m && a.ld_w >= la_div(row_w, m) * m && (a.ld_x * e) % 16 == 0 && (a.ld_w * e) % 16 == 0 &&
          hotk_aligned16(a.x) && hotk_aligned16(a.w);
 }
-LaShape la_shape(const hotk_linear_args& a) { return la_shape(a.M, a.N, a.K, a.type, a.out_type, a.flags & (HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN), la_whole(a), a.x_lo ? 2 : 1); }
+LaShape la_shape(const hotk_linear_args& a) {
+  const int64_t e = ffn_bytes(a.type);
+  const bool off_word = (((uintptr_t)a.x | (uintptr_t)a.w | (uint64_t)(a.ld_x * e) | (uint64_t)(a.ld_w * e)) & 3) != 0;
+  return la_shape(a.M, a.N, a.K, a.type, a.out_type, a.flags & (HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN), la_whole(a), off_word, a.x_lo ? 2 : 1);
+}
 
 int la_check(const hotk_linear_args& a) {
   HOTK_CHECK_ARG(a.M >= 0 && a.N > 0 && a.K > 0);

@@ -839,3 +839,32 @@ def test_scales_far_apart(M, dt):
     sx[0], sw[1] = float('nan'), float('nan')
     got = ops.linear_act_quantized(xq, sx, wq, sw, out_dtype=dt)
     assert got[0].isnan().all() and got[:, 1].isnan().all() and got[1:, 2:].isfinite().all()
+
+
+@pytest.mark.parametrize('M', [1, 16, 20, 64])
+@pytest.mark.parametrize('K', [1, 15, 17, 131, 1029])
+def test_few_rows_off_a_words_start(M, K):
+    """rows that start at each byte of a word (8 bits) or at its middle (16 bits), last ones at their tensor's end, NaN around them"""
+    from hot_amd import ops
+    N = 21
+    for start in range(4):
+        for pad in (0, 1, 2, 5):                                     # the rows' stride goes through all bytes too
+            def rows8(seed, n):
+                flat = torch.full((start + n * (K + pad),), float('nan'), device=DEV).to(E4M3)
+                view = flat[start:].view(n, K + pad)[:, :K]
+                view.copy_(rnd(seed, n, K).to(E4M3))
+                return view
+            xq, wq, sx, sw = rows8(450, M), rows8(451, N), rnd(452, M).abs() + 0.1, rnd(453, N).abs() + 0.1
+            got = ops.linear_act_quantized(xq, sx, wq, sw, out_dtype=torch.float32)
+            scale = sx.double()[:, None] * sw.double()
+            want, size = (xq.double() @ wq.double().t()) * scale, (xq.double().abs() @ wq.double().abs().t()) * scale
+            hold('8 bits', got, want, half_step(torch.float32) * want.abs() + (K + 4) * E * size)
+            for dt in (torch.bfloat16, torch.float16):
+                def rows16(seed, n):
+                    flat = torch.full((start + n * (K + pad),), float('nan'), device=DEV, dtype=dt)
+                    view = flat[start:].view(n, K + pad)[:, :K]
+                    view.copy_(rnd(seed, n, K).to(dt))
+                    return view
+                x, w = rows16(454, M), rows16(455, N)
+                want = x.double() @ w.double().t()
+                hold('16 bits', ops.linear_act(x, w), want, half_step(dt) * want.abs() + (K + 2) * E * (x.double().abs() @ w.double().abs().t()) + floor_of(dt))
