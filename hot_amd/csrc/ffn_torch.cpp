@@ -115,6 +115,12 @@ int type_of(at::ScalarType t) {
   }
 }
 
+// derivatives are of first order and in reverse: a tensor that carries a forward derivative would lose it here
+void check_tangent(const Tensor& t, const char* what) {
+  if (t.defined() && t._fw_grad(/*level=*/0).defined())
+    refuse(what, " carries a forward-mode derivative: there are gradients in reverse mode only");
+}
+
 // the values are what the memory holds
 void check_memory(const Tensor& t, const char* what) {
   if (t.layout() != at::kStrided) refuse(what, ": a strided tensor is expected");
@@ -123,6 +129,7 @@ void check_memory(const Tensor& t, const char* what) {
 
 void check_input(const Tensor& x, const char* what, bool eight = false) {
   if (!x.defined()) refuse(what, ": a tensor is expected");
+  check_tangent(x, what);
   if (!x.is_cuda())
     refuse("hot_amd kernels run on a HIP device only; ", what, " is on ", x.device(), ". There is no CPU path: move it to the GPU.");
   const int ty = type_of(x.scalar_type());
@@ -135,6 +142,7 @@ void check_input(const Tensor& x, const char* what, bool eight = false) {
 // an operand that goes with `ref`: on its device, of this type and shape
 void check_with(const Tensor& ref, const Tensor& t, const char* what, at::IntArrayRef shape, at::ScalarType type) {
   if (!t.defined()) refuse(what, ": a tensor is expected");
+  check_tangent(t, what);
   if (t.device() != ref.device()) refuse(what, " is on ", t.device(), ", the input on ", ref.device());
   if (t.scalar_type() != type) refuse(what, ": ", type, " expected, got ", t.scalar_type());
   check_memory(t, what);
@@ -183,8 +191,9 @@ void refuse_grad(const char* what, const T&... t) {
   if (at::GradMode::is_enabled() && (wants_grad(t) || ...))
     refuse(what, " has no gradient: call it under torch.no_grad() or on detached tensors");
 }
-void first_order(const char* what) {
+void first_order(const char* what, const variable_list& gradients) {
   if (at::GradMode::is_enabled()) refuse(what, " has gradients of first order only (create_graph=True asks for more)");
+  for (const Tensor& g : gradients) check_tangent(g, "a gradient");
 }
 
 // ---- norm --------------------------------------------------------------------------------------------------------------
@@ -237,7 +246,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     return {o.y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    first_order("rms_norm");
+    first_order("rms_norm", g);
     const auto saved = ctx->get_saved_variables();
     const Tensor &h = saved[0], &rstd = saved[1], &w = saved[2], &kind = saved[3];
     const int64_t wants = ctx->saved_data["wants"].toInt(), keep = ctx->saved_data["keep"].toInt();
@@ -436,7 +445,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    first_order("linear_act");
+    first_order("linear_act", g);
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &save = saved[2], &dy = g[0];
     const int act = (int)ctx->saved_data["act"].toInt();
