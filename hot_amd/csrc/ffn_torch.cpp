@@ -117,8 +117,18 @@ int type_of(at::ScalarType t) {
 
 // derivatives are of first order and in reverse: a tensor that carries a forward derivative would lose it here
 void check_tangent(const Tensor& t, const char* what) {
-  if (t.defined() && t._fw_grad(/*level=*/0).defined())
+  if (t._fw_grad(/*level=*/0).defined())
     refuse(what, " carries a forward-mode derivative: there are gradients in reverse mode only");
+}
+
+// a tensor with memory of its own: one that stands for others (under torch.func's transforms, a class with __torch_dispatch__
+// such as a distributed or a fake tensor) has none, and an optional operand without memory would count as one not given
+void check_plain(const Tensor& t, const char* what) {
+  using c10::DispatchKey;
+  if (t.key_set().has_any(c10::DispatchKeySet({DispatchKey::Python, DispatchKey::Batched, DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper,
+                                                  DispatchKey::Functionalize})))
+    refuse(what, ": a plain tensor is expected, not one that stands for others (torch.func, vmap, __torch_dispatch__)");
+  check_tangent(t, what);
 }
 
 // the values are what the memory holds
@@ -129,7 +139,7 @@ void check_memory(const Tensor& t, const char* what) {
 
 void check_input(const Tensor& x, const char* what, bool eight = false) {
   if (!x.defined()) refuse(what, ": a tensor is expected");
-  check_tangent(x, what);
+  check_plain(x, what);
   if (!x.is_cuda())
     refuse("hot_amd kernels run on a HIP device only; ", what, " is on ", x.device(), ". There is no CPU path: move it to the GPU.");
   const int ty = type_of(x.scalar_type());
@@ -142,7 +152,7 @@ void check_input(const Tensor& x, const char* what, bool eight = false) {
 // an operand that goes with `ref`: on its device, of this type and shape
 void check_with(const Tensor& ref, const Tensor& t, const char* what, at::IntArrayRef shape, at::ScalarType type) {
   if (!t.defined()) refuse(what, ": a tensor is expected");
-  check_tangent(t, what);
+  check_plain(t, what);
   if (t.device() != ref.device()) refuse(what, " is on ", t.device(), ", the input on ", ref.device());
   if (t.scalar_type() != type) refuse(what, ": ", type, " expected, got ", t.scalar_type());
   check_memory(t, what);
@@ -193,7 +203,8 @@ void refuse_grad(const char* what, const T&... t) {
 }
 void first_order(const char* what, const variable_list& gradients) {
   if (at::GradMode::is_enabled()) refuse(what, " has gradients of first order only (create_graph=True asks for more)");
-  for (const Tensor& g : gradients) check_tangent(g, "a gradient");
+  for (const Tensor& g : gradients)
+    if (g.defined()) check_plain(g, "a gradient");
 }
 
 // ---- norm --------------------------------------------------------------------------------------------------------------
@@ -205,6 +216,7 @@ void check_norm(const Tensor& x, const Tensor& w, const optional<Tensor>& r, con
   if (L.rmsnorm_supported(D, type_of(x.scalar_type())) != 1) refuse("rows of up to 32768 elements are normalised, got ", D);
   if (keep < 0 || keep > 0xffffffffll) refuse("keep: a bit set over kinds expected, got ", keep);
   if (!(eps >= 0.)) refuse("eps: a number >= 0 expected, got ", eps);
+  if (kind && kind->defined()) check_plain(*kind, "kind");
   if (kind && (!kind->defined() || kind->scalar_type() != at::kByte || kind->numel() != x.numel() / D || kind->device() != x.device()))
     refuse("kind: uint8, one per row (", x.numel() / D, "), on ", x.device(), " expected");
 }

@@ -6,7 +6,8 @@ Tensors are fp32, bf16 or fp16 on one HIP device, [..., width], read in place wh
 new, contiguous tensors.  Sums, statistics and epilogues are in 32 bits and every result is rounded once.  Launches go to the
 current stream of the tensors' device; workspaces come from torch's allocator per call, so calls can be captured into a
 graph and captured graphs share nothing.  Gradients are of first order and in reverse mode; create_graph=True is refused in the backward pass, and tensors that carry a
-forward-mode derivative (torch.autograd.forward_ad) everywhere."""
+forward-mode derivative (torch.autograd.forward_ad) everywhere, as are tensors that stand for others (torch.func, vmap, classes
+with __torch_dispatch__)."""
 import torch
 
 from . import _lib

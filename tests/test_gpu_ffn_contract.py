@@ -38,3 +38,28 @@ def test_forward_derivatives_are_refused():
             with pytest.raises(RuntimeError, match='forward-mode'):
                 torch.autograd.grad(y, leaf, d(torch.ones_like(y)))
         assert torch.equal(ops.rms_norm(x, w), ops.rms_norm(leaf, w).detach())       # within the level, without a derivative: as ever
+
+
+def test_tensors_that_stand_for_others_are_refused():
+    """in any place: an optional operand without memory would otherwise count as none, a batched gradient as one"""
+    from hot_amd import ops
+    from hot_amd._lib import HotkError
+    from test_ffn_refusals import Wrapped
+    x, w, W, b, y = rnd(510, 6, 16), rnd(511, 16), rnd(512, 24, 16), rnd(513, 24), rnd(514, 6, 24)
+    kind = torch.ones(6, dtype=torch.uint8, device=DEV)
+    q, s = ops.quantize_rows(x)
+    wq, ws = ops.quantize_rows(W)
+    v = Wrapped
+    calls = [lambda: ops.rms_norm(v(x), w), lambda: ops.rms_norm(x, v(w)), lambda: ops.rms_norm(x, w, v(x)), lambda: ops.rms_norm(x, w, kind=v(kind)),
+             lambda: ops.rms_norm_quantized(x, w, v(x)), lambda: ops.quantize_rows(v(x)), lambda: ops.linear_act(x, v(W)),
+             lambda: ops.linear_act(x, W, v(b)), lambda: ops.linear_act(x, W, residual=v(y)), lambda: ops.linear_act_quantized(v(q), s, wq, ws),
+             lambda: ops.linear_act_quantized(q, v(s), wq, ws), lambda: ops.linear_act_quantized(q, s, wq, v(ws)),
+             lambda: ops.linear_act_quantized(q, s, wq, ws, v(b), out_dtype=torch.float32)]
+    for i, call in enumerate(calls):
+        with pytest.raises(HotkError, match='plain tensor'):
+            call()
+            raise AssertionError(f'call {i} was taken')
+    leaf = x.clone().requires_grad_(True)
+    for z in (ops.rms_norm(leaf, w), ops.linear_act(leaf, W, act='silu')):
+        with pytest.raises(RuntimeError, match='plain tensor'):
+            torch.autograd.grad(z, leaf, torch.ones(3, *z.shape, device=DEV), is_grads_batched=True)
