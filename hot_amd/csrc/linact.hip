@@ -54,19 +54,23 @@ constexpr int64_t LA_MAX_GRID = 1 << 23;           // workgroups of up to 512 th
 __device__ __align__(16) const uint32_t la_zeros[4] = {0, 0, 0, 0};   // what lies past the end of a contraction
 
 // ---- activations: f(z) and f'(z) ---------------------------------------------------------------------------------------
-// FAST (16-bit results): gelu by Abramowitz & Stegun 7.1.26 (|error of erf| <= 1.5e-7), whose exponential the slope shares;
-// tanh and the logistic function from one exponential.  fp32 results: gelu by the Chebyshev fit of erfc in Press et al.,
-// Numerical Recipes, 6.2 (relative error below 1.2e-7; a third of the library function's time), else the math library.
+// FAST (16-bit results): gelu from q = erfc(|z| / sqrt 2) / 2 = exp(-z^2 / 2) P(t), t = 1 / (1 + p |z|), whose exponential the slope
+// shares; p and the sixth-degree P, without a constant, were fitted here (weighted least squares, weights by the last fit's
+// error) so that q as computed is off by less than 3e-7 and less than 3e-5 of itself: the negative tail, z q, is as exact as the type
+// holds it.  tanh and the logistic function from one exponential.  fp32 results: gelu by the Chebyshev fit of erfc in Press
+// et al., Numerical Recipes, 6.2 (relative error below 1.2e-7, and 1.5 z^2 2^-24 from the exponent's own rounding; a third of
+// the library function's time), else the math library.
 // ACT: HOTK_ACT_RELU stands for all three that are linear on either side of zero, with `neg` the slope below it.
 template <int ACT, bool FAST>
 __device__ __forceinline__ float la_act(float z, float neg, float& slope) {
   if constexpr (ACT == HOTK_ACT_GELU) {
     float cdf, pdf;
-    if (FAST) {            // q = half of erfc(|z| / sqrt 2), cdf = 1/2 + sign(z) (1/2 - q)
-      const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
+    if (FAST) {
+      const float t = __builtin_amdgcn_rcpf(fmaf(0.2958828887f, fabsf(z), 1.f));
       const float e = __builtin_amdgcn_exp2f(z * (-0.72134752f * z));
-      const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f) * e;
-      cdf = 0.5f + copysignf(0.5f - q, z);
+      const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, -0.08316676316f, 0.2464154638f), -0.04891132795f), 0.1582405465f), 0.1087127227f),
+                               0.1187092262f) * e;
+      cdf = z < 0.f ? q : 1.f - q;       // (1/2 - (1/2 - q) would leave nothing of a small q)
       pdf = 0.39894228f * e;
     } else {
       const float x = 0.70710678f * fabsf(z), xx = 0.5f * z * z;
@@ -74,7 +78,7 @@ __device__ __forceinline__ float la_act(float z, float neg, float& slope) {
       const float p = fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.17087277f, -0.82215223f), 1.48851587f), -1.13520398f),
                       0.27886807f), -0.18628806f), 0.09678418f), 0.37409196f), 1.00002368f), -1.26551223f);
       const float q = 0.5f * t * __builtin_amdgcn_exp2f(1.44269504f * (p - xx));
-      cdf = 0.5f + copysignf(0.5f - q, z);
+      cdf = z < 0.f ? q : 1.f - q;
       pdf = 0.39894228f * __builtin_amdgcn_exp2f(-1.44269504f * xx);
     }
     slope = fmaf(z, pdf, cdf);

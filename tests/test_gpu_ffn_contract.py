@@ -4,7 +4,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
-from test_gpu_ffn import DEV, rnd
+from test_gpu_ffn import DEV, E, TYPES, act64, floor_of, half_step, hold, rnd, slope64
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,47 @@ def test_tensors_that_stand_for_others_are_refused():
     for z in (ops.rms_norm(leaf, w), ops.linear_act(leaf, W, act='silu')):
         with pytest.raises(RuntimeError, match='plain tensor'):
             torch.autograd.grad(z, leaf, torch.ones(3, *z.shape, device=DEV), is_grads_batched=True)
+
+
+# ------------------------------------------------------------------------------------------------
+# activations far from zero
+# ------------------------------------------------------------------------------------------------
+def column(z, n, dt):
+    """operands whose product is z in each of n columns, exactly: one term, times one"""
+    return z.to(dt)[:, None].to(DEV), torch.ones(n, 1, dtype=dt, device=DEV)
+
+
+# gelu(z) = z q, q = erfc(-z / sqrt 2) / 2.  16-bit results: q's fit to 3e-5 of itself below z = -2.6 (q < 0.0047); fp32: to 1.2e-7.
+# The exponent z^2 / 2 has up to three roundings, 1.5 z^2 E of the result, and sixteen operations besides.
+def gelu_tail(z, dt):
+    return 1.2e-7 + (0 if dt == torch.float32 else 3e-5) + (1.5 * z * z + 16) * E
+
+
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('M', [33, 400])
+def test_gelu_negative_tail(M, dt):
+    """relative to its value, down to where the type ends, in both kernels and over 8-bit operands"""
+    from hot_amd import ops
+    x, w = column(-torch.linspace(2.6, 12.5, M), 24, dt)
+    z = x.double().expand(M, 24)
+    want = act64(z, 'gelu')
+    hold('y', ops.linear_act(x, w, act='gelu'), want, (half_step(dt) + gelu_tail(z, dt)) * want.abs() + floor_of(dt))
+    e = (-torch.linspace(2.6, 12.5, M)).to(torch.float8_e4m3fn)[:, None].to(DEV)
+    z = e.double().expand(M, 24)
+    want = act64(z, 'gelu')
+    one = torch.ones(24, device=DEV)
+    got = ops.linear_act_quantized(e, torch.ones(M, device=DEV), one[:, None].to(torch.float8_e4m3fn), one, act='gelu', out_dtype=dt)
+    hold('8 bits', got, want, (half_step(dt) + gelu_tail(z, dt)) * want.abs() + floor_of(dt))
+
+
+@pytest.mark.parametrize('M', [33, 400])
+def test_gelu_gradient_in_the_negative_tail(M):
+    """fp32: slope = q + z exp(-z^2 / 2) / sqrt(2 pi); the second term dominates and has the exponent's roundings too"""
+    from hot_amd import ops
+    x, w = column(-torch.linspace(2.6, 12.5, M), 1, torch.float32)
+    x.requires_grad_(True)
+    y = ops.linear_act(x, w, act='gelu')
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    z = x.detach().double()
+    want = slope64(z, 'gelu')
+    hold('dx', dx, want, 3 * gelu_tail(z, torch.float32) * want.abs() + floor_of(torch.float32))
