@@ -84,18 +84,14 @@ __device__ __forceinline__ float la_act(float z, float neg, float& slope) {
     slope = fmaf(z, pdf, cdf);
     return z * cdf;
   } else if constexpr (ACT == HOTK_ACT_TANH) {
-    float t;
-    if (FAST) {
-      const float s = z * z;
-      const float series = z * fmaf(s, fmaf(s, fmaf(s, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);   // to z^7: |z| < 1/4
-      const float e = __builtin_amdgcn_exp2f(2.88539008f * z);
-      const float quot = fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
-      t = fabsf(z) < 0.25f ? series : quot;
-    } else {
-      t = tanhf(z);
-    }
-    slope = fmaf(-t, t, 1.f);
-    return t;
+    // q = 1 - |tanh z| = 2 / (e^2|z| + 1): the slope 1 - tanh^2 is q (2 - q), which keeps its digits where tanh is next to one
+    const float e = FAST ? __builtin_amdgcn_exp2f(2.88539008f * fabsf(z)) : expf(2.f * fabsf(z));
+    const float q = FAST ? 2.f * __builtin_amdgcn_rcpf(e + 1.f) : 2.f / (e + 1.f);
+    slope = q * (2.f - q);
+    if (!FAST) return tanhf(z);
+    const float s = z * z;
+    const float series = z * fmaf(s, fmaf(s, fmaf(s, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);   // to z^7: |z| < 1/4
+    return fabsf(z) < 0.25f ? series : copysignf(1.f - q, z);
   } else if constexpr (ACT == HOTK_ACT_SILU) {
     const float e = FAST ? __builtin_amdgcn_exp2f(-1.44269504f * z) : expf(-z);
     const float s = FAST ? __builtin_amdgcn_rcpf(1.f + e) : 1.f / (1.f + e);

@@ -107,3 +107,16 @@ def test_gelu_gradient_in_the_negative_tail(M):
     z = x.detach().double()
     want = slope64(z, 'gelu')
     hold('dx', dx, want, 3 * gelu_tail(z, torch.float32) * want.abs() + floor_of(torch.float32))
+
+
+@pytest.mark.parametrize('M', [33, 400])
+def test_tanh_gradient_far_from_zero(M):
+    """fp32: the slope 1 / cosh^2 relative to its value, where 1 - tanh^2 has no digits left; the exponent 2 |z| is rounded once, and
+    a dozen operations follow"""
+    from hot_amd import ops
+    x, w = column(torch.linspace(-40, 40, M), 1, torch.float32)
+    x.requires_grad_(True)
+    y = ops.linear_act(x, w, act='tanh')
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    z = x.detach().double()
+    hold('dx', dx, z.cosh() ** -2, (2 * z.abs() + 12) * E * z.cosh() ** -2 + floor_of(torch.float32))
