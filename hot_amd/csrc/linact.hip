@@ -26,9 +26,9 @@
 // 1 362 TFLOP/s, 8 192^3 e4m3 389 us = 2 823; 16 384 x 4 096 x 1 024 bf16 129 us = 1 066 (with bias, gelu and slopes 184), its
 // dx 111 us = 1 238, its dw 135 us = 1 018; 8 192 x 2 048 x 4 096 e4m3 62 us = 2 200; 4 096 x 4 096 x 1 024 fp32 254 us = 135.
 //
-// For training, 16-bit types keep f'(z) as a 16-bit fixed-point number in steps of 2^-14 (|f'| < 1.13): its error of 2^-15
-// is far below the rounding of dz, where z rounded to the type would add as much as that rounding again, and the backward
-// pass needs no transcendental.  fp32 keeps z.
+// For training, 16-bit types keep f'(z) in a 16-bit code (la_slope_codes) whose error stays below what dz's own rounding adds,
+// where z rounded to the type would add as much again and more as |z| grows, and the backward pass needs no transcendental.
+// fp32 keeps z.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -45,7 +45,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-constexpr float LA_SLOPE_STEP = 0x1p-14f;
 constexpr int LA_SLOPE_NAN = -32768;
 constexpr float LA_LEAK = 0.01f;
 constexpr int LA_MAX_SPLIT = 16;
@@ -121,28 +120,65 @@ __device__ __forceinline__ void la_times_slope(f32x4& v, const f32x4& z, int act
     default: each(std::integral_constant<int, HOTK_ACT_RELU>{});
   }
 }
-// eight slopes in steps of 2^-14 (the packed conversion's unit is 1 / 32767); a NaN among them is rare, and looked for in their sum
+// Codes of slopes, -0.13 < d < 1.13.  A code is sign(d) k - 8192: the codes below zero that negative slopes leave unused go to the
+// positive ones.  From |d| = 1/16 up k goes in steps of 2^-14 (2^-11 of |d| at most); below, where a saturated unit's gradient
+// lives, as a root of |d|, so that k's half step stays small against |d|:  k = 21504 (16 |d|)^(1/n).  fp16: n = 8, half a step is
+// 2^-12.4 of |d| at 1/16, 2^-11.2 at 2^-14 (fp16's smallest normal number), 2^-10 at 2^-23; bf16: n = 16, 2^-11.4 at 1/16, 2^-10 at
+// 2^-26, 2^-8 at 2^-58.  The types' own half steps are 2^-11 and 2^-8.  (With one step of 2^-14 for all, at the cost of two
+// transcendentals less, gradients of tanh units were 9 % off at |z| = 5.5 and zero from 6 on.)  Piecewise linear activations
+// need one bit.
 typedef int16_t s16x8 __attribute__((ext_vector_type(8)));
+constexpr float LA_CODE_EDGE = 0.0625f, LA_CODE_AT_EDGE = 21504.f, LA_CODE_SHIFT = 8192.f, LA_CODE_STEP = 0x1p-14f;
+template <class OT> struct LaRoot;
+template <> struct LaRoot<_Float16> {
+  static constexpr int N = 8;
+  static constexpr float LOG_EDGE = -0.10763855f;      // log2(21504 / 32767 * 16^(1/n)): the packed conversion's unit is 1 / 32767
+  static constexpr float WEIGHT = 0.70710678f / LA_CODE_AT_EDGE;       // 16^(-1/n)
+};
+template <> struct LaRoot<__bf16> {
+  static constexpr int N = 16;
+  static constexpr float LOG_EDGE = -0.35763855f;
+  static constexpr float WEIGHT = 0.84089642f / LA_CODE_AT_EDGE;
+};
+template <int ACT, class OT>
 __device__ __forceinline__ s16x8 la_slope_codes(const float* d) {
-  constexpr float UNIT = 16384.f / 32767.f;
+  constexpr float UNIT = 1.f / 32767.f;
   s16x8 c;
-  float sum = 0.f;
+  if constexpr (ACT == HOTK_ACT_RELU) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) c[k] = d[k] == 1.f;
+    return c;
+  }
+  float sum = 0.f, v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float a = fabsf(d[k]);
+    const float linear = fmaf(a, UNIT / LA_CODE_STEP, UNIT * (LA_CODE_AT_EDGE - LA_CODE_EDGE / LA_CODE_STEP));
+    const float root = __builtin_amdgcn_exp2f(fmaf(__builtin_amdgcn_logf(a), 1.f / LaRoot<OT>::N, LaRoot<OT>::LOG_EDGE));
+    v[k] = copysignf(a < LA_CODE_EDGE ? root : linear, d[k]) - UNIT * LA_CODE_SHIFT;
+    sum += d[k];
+  }
 #pragma unroll
   for (int k = 0; k < 8; k += 2) {
-    const auto p = __builtin_amdgcn_cvt_pknorm_i16(d[k] * UNIT, d[k + 1] * UNIT);
+    const auto p = __builtin_amdgcn_cvt_pknorm_i16(v[k], v[k + 1]);
     c[k] = p[0];
     c[k + 1] = p[1];
-    sum += d[k] + d[k + 1];
   }
-  if (sum != sum) {
+  if (sum != sum) {                      // (a NaN among them is rare)
 #pragma unroll
     for (int k = 0; k < 8; ++k) c[k] = d[k] != d[k] ? (int16_t)LA_SLOPE_NAN : c[k];
   }
   return c;
 }
+template <class OT>
 __device__ __forceinline__ float la_slope(int16_t code, int act) {
-  if (act == HOTK_ACT_LEAKYRELU) return code > 8192 ? 1.f : LA_LEAK;
-  return code == LA_SLOPE_NAN ? __builtin_nanf("") : (float)code * LA_SLOPE_STEP;
+  if (act == HOTK_ACT_RELU || act == HOTK_ACT_LEAKYRELU) return code ? 1.f : la_neg(act);
+  const float c = (float)code + LA_CODE_SHIFT, a = fabsf(c);
+  float root = a * LaRoot<OT>::WEIGHT;
+#pragma unroll
+  for (int n = LaRoot<OT>::N; n > 1; n /= 2) root *= root;
+  const float linear = fmaf(a, LA_CODE_STEP, LA_CODE_EDGE - LA_CODE_AT_EDGE * LA_CODE_STEP);
+  return code == LA_SLOPE_NAN ? __builtin_nanf("") : copysignf(a < LA_CODE_AT_EDGE ? root : linear, c);
 }
 
 // ---- epilogue ----------------------------------------------------------------------------------------------------------
@@ -171,12 +207,13 @@ __device__ __forceinline__ void la_activate(const LaEpi<OT>& e, int64_t m, int64
   }
 #pragma unroll
   for (int i = 0; i < W; ++i) z[i] = la_act<ACT, FAST>(z[i], neg, d[i]);
-  if (FAST && e.save && e.act != HOTK_ACT_NONE) {
+  if constexpr (FAST) {
+    if (!e.save || e.act == HOTK_ACT_NONE) return;
     typedef int16_t s16x8u __attribute__((ext_vector_type(8), aligned(2)));
     int16_t* row = (int16_t*)e.save + m * N + n0;
 #pragma unroll
     for (int i = 0; i < W; i += 8) {
-      const s16x8 c = la_slope_codes(d + i);
+      const s16x8 c = la_slope_codes<ACT, OT>(d + i);
       if (i + 8 <= left) {
         *reinterpret_cast<s16x8u*>(row + i) = c;
       } else {
@@ -706,11 +743,11 @@ __global__ __launch_bounds__(256) void k_linact_dz(const T* __restrict__ in, int
             if (WHOLE) {
               const s16x8u d = *reinterpret_cast<const s16x8u*>(codes);
 #pragma unroll
-              for (int k = 0; k < E::VEC; ++k) v[k] *= la_slope(d[k], act);
+              for (int k = 0; k < E::VEC; ++k) v[k] *= la_slope<T>(d[k], act);
             } else {
 #pragma unroll
               for (int k = 0; k < E::VEC; ++k)
-                if (k < left) v[k] *= la_slope(codes[k], act);
+                if (k < left) v[k] *= la_slope<T>(codes[k], act);
             }
           }
         }

@@ -120,3 +120,73 @@ def test_tanh_gradient_far_from_zero(M):
     dx, = torch.autograd.grad(y, x, torch.ones_like(y))
     z = x.detach().double()
     hold('dx', dx, z.cosh() ** -2, (2 * z.abs() + 12) * E * z.cosh() ** -2 + floor_of(torch.float32))
+
+
+SMOOTH = ['gelu', 'tanh', 'silu']
+
+
+def slope64_far(z, act):
+    """slopes in 64 bits that keep their digits where the activation saturates"""
+    s = torch.sigmoid(z)
+    return {'gelu': lambda: slope64(z, 'gelu'), 'tanh': lambda: z.cosh() ** -2, 'silu': lambda: s * (1 + z * torch.sigmoid(-z))}[act]()
+
+
+def code_error(s, dt):
+    """half a step of the 16-bit code of a slope: 2^-15 from 1/16 up; below, the code is 21504 (16 |s|)^(1/n), whose half step is
+    n / (2 code) of s (a tenth more for the curve within it)"""
+    a, n = s.abs(), 8 if dt == torch.float16 else 16
+    return torch.where(a >= 1 / 16, torch.full_like(a, 2.0 ** -15), 1.1 * a * n / (2 * 21504 * (16 * a) ** (1 / n)).clamp_min(1e-300))
+
+
+def slope_error(z, s, act):
+    """a 16-bit slope as computed: gelu's fit to 3e-5 of q (below |slope|, |z| > 2.6), a few operations next to an exponent that is
+    rounded up to three times; where a slope crosses zero or q is large, 32-bit operations of size one"""
+    return ((3e-5 if act == 'gelu' else 0) + (1.5 * z * z + 2 * z.abs() + 32) * E) * s.abs() + torch.where(z.abs() < 2.7, 1e-6, 0.)
+
+
+@pytest.mark.parametrize('dt', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('act', SMOOTH)
+@pytest.mark.parametrize('M', [33, 400])
+def test_gradients_of_saturated_units(M, act, dt):
+    """|z| up to 12: the gradient relative to its value, down to where the type ends"""
+    from hot_amd import ops
+    x, w = column(torch.linspace(-12, 12, M), 1, dt)
+    z = x.double()
+    s = slope64_far(z, act)
+    for scale in (1., 256.):                       # (a scaled loss lifts what fp16 could not hold)
+        leaf, b = x.clone().requires_grad_(True), torch.zeros(1, dtype=dt, device=DEV, requires_grad=True)
+        y = ops.linear_act(leaf, w, b, act=act)
+        dx, db = torch.autograd.grad(y, (leaf, b), torch.full_like(y, scale))
+        want, off = scale * s, scale * (code_error(s, dt) + slope_error(z, s, act))
+        hold('dx', dx, want, half_step(dt) * (want.abs() + off) + off + 2 * floor_of(dt))
+        hold('db', db, want.sum(0), half_step(dt) * want.sum(0).abs() + off.sum(0) + (M + 8) * E * want.abs().sum(0) + floor_of(dt))
+
+
+@pytest.mark.parametrize('dt', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('act,bias', [('silu', -10.), ('tanh', 6.), ('tanh', -6.), ('gelu', -4.5)])
+@pytest.mark.parametrize('M,N,K', [(900, 40, 160), (4096, 64, 160)])
+def test_weight_gradients_of_saturated_units(M, N, K, act, bias, dt):
+    """a layer whose units sit far from zero: dx and dw are off by the roundings of dz (one, where the product is long) and of the
+    result, each at most 0.58 u as a whole, and by the slope's code"""
+    from hot_amd import ops
+    x, w, b = rnd(520, M, K, dt=dt), rnd(521, N, K, dt=dt, scale=0.5 * K ** -0.5), torch.full((N,), bias, dtype=dt, device=DEV)
+    dy = rnd(522, M, N, dt=dt, scale=1. if dt == torch.bfloat16 else 4096.)
+    z = x.double() @ w.double().t() + b.double()
+    s = slope64_far(z, act)
+    dz = dy.double() * s
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(ops.linear_act(*leaves, act=act), leaves, dy)
+    u = 0.58 * half_step(dt)
+    code = float((dy.double() * code_error(s, dt)).norm() / dz.norm()) * 0.58 + float(((K + 8) * E * z.abs() + 1e-5).max())
+    for what, got, want, roundings in (('dx', dx, dz @ w.detach().double(), 2), ('dw', dw, dz.t() @ x.detach().double(), 2), ('db', db, dz.sum(0), 1)):
+        assert float((got.double() - want).norm() / want.norm()) <= (roundings * u * u + code * code) ** 0.5, what
+
+
+def test_piecewise_linear_slopes_are_exact():
+    from hot_amd import ops
+    for dt in (torch.bfloat16, torch.float16):
+        x, w = column(torch.tensor([-3., -1e-3, 0., 1e-3, 5.]), 1, dt)
+        for act, low in (('relu', 0.), ('leakyrelu', 0.01)):
+            leaf = x.clone().requires_grad_(True)
+            dx, = torch.autograd.grad(ops.linear_act(leaf, w, act=act), leaf, torch.ones(5, 1, dtype=dt, device=DEV))
+            assert torch.equal(dx[:, 0], torch.tensor([low, low, low, 1., 1.]).to(dt).to(DEV))
