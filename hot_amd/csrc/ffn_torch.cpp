@@ -159,6 +159,15 @@ void check_with(const Tensor& ref, const Tensor& t, const char* what, at::IntArr
   if (t.sizes() != shape) refuse(what, ": shape ", shape, " expected, got ", t.sizes());
 }
 
+// what the forward pass kept as memory of `n` elements in a row, as the backward pass finds it: a saved-tensor hook may have put another
+// tensor in its place, so its values are taken in any layout, and anything but n values of this type beside `ref` is refused
+Tensor kept_values(const Tensor& ref, const Tensor& t, const char* what, int64_t n, at::ScalarType type) {
+  if (!t.defined()) refuse(what, " kept for the backward pass did not come back");
+  check_with(ref, t, what, t.sizes(), type);
+  if (t.numel() != n) refuse(what, " kept for the backward pass came back with ", t.numel(), " elements instead of ", n);
+  return t.contiguous();
+}
+
 // [..., C] as rows in place: the tensor, elements from row to row, rows; a copy where the rows lie at no single stride
 struct Rows {
   Tensor t;
@@ -253,21 +262,26 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     Normed o = norm_forward(x, weight, r, kind, keep, eps, true);
     ctx->save_for_backward({r ? o.h : x, o.rstd, o.w, o.kind});
     ctx->saved_data["keep"] = keep;
-    ctx->saved_data["wants"] = (int64_t)(wants_grad(x) | wants_grad(weight) << 1 | wants_grad(r) << 2 | (r ? 1 : 0) << 3);
+    ctx->saved_data["wants"] = (int64_t)(wants_grad(x) | wants_grad(weight) << 1 | wants_grad(r) << 2 | (r ? 1 : 0) << 3 | (kind ? 1 : 0) << 4);
     if (r) return {o.y, o.h};
     return {o.y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     first_order("rms_norm", g);
     const auto saved = ctx->get_saved_variables();
-    const Tensor &h = saved[0], &rstd = saved[1], &w = saved[2], &kind = saved[3];
     const int64_t wants = ctx->saved_data["wants"].toInt(), keep = ctx->saved_data["keep"].toInt();
     const bool has_r = wants & 8;
     Tensor dy = g[0], dh = has_r ? g[1] : Tensor(), dx, dw;
     if (dy.defined() || dh.defined()) {
-      const c10::DeviceGuard guard(h.device());
-      const int ty = type_of(h.scalar_type());
-      const int64_t D = h.size(-1);
+      const Tensor& ref = dy.defined() ? dy : dh;      // of the rows' device, type and shape
+      const c10::DeviceGuard guard(ref.device());
+      const auto type = ref.scalar_type();
+      const int ty = type_of(type);
+      const int64_t D = ref.size(-1), n = ref.numel() / D;
+      const Tensor& h = saved[0];
+      check_with(ref, h, "the stream", ref.sizes(), type);
+      const Tensor rstd = kept_values(ref, saved[1], "a norm's statistics", n, at::kFloat), w = kept_values(ref, saved[2], "weight", D, type);
+      const Tensor kind = wants & 16 ? kept_values(ref, saved[3], "kind", n, at::kByte) : Tensor();
       if (!dy.defined()) dy = at::zeros_like(h);
       const Rows hs = rows(h), gs = rows(dy), ss = dh.defined() ? rows(dh) : Rows{};
       void* st = stream_of(h);
@@ -459,17 +473,21 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     first_order("linear_act", g);
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &weight = saved[1], &save = saved[2], &dy = g[0];
+    const Tensor& dy = g[0];
     const int act = (int)ctx->saved_data["act"].toInt();
     const int64_t wants = ctx->saved_data["wants"].toInt();
     const auto shape = ctx->saved_data["shape"].toIntVector(), ld = ctx->saved_data["ld"].toIntVector();
-    const int64_t K = shape.back(), N = weight.size(0);
-    int64_t M = 1;
-    for (size_t i = 0; i + 1 < shape.size(); ++i) M *= shape[i];
     Tensor dx, dw, db;
     if (dy.defined() && (wants & 7)) {
-      const c10::DeviceGuard guard(x.device());
-      const auto type = x.scalar_type();
+      const c10::DeviceGuard guard(dy.device());
+      const auto type = dy.scalar_type();
+      const int64_t K = shape.back(), N = dy.size(-1), M = dy.numel() / N;
+      // the operands: themselves in any layout, or copies of rows `ld` apart
+      if (!ld[0]) check_with(dy, saved[0], "x", shape, type);
+      if (!ld[1]) check_with(dy, saved[1], "weight", {N, K}, type);
+      const Tensor x = ld[0] ? kept_values(dy, saved[0], "x", M * ld[0], type) : saved[0];
+      const Tensor weight = ld[1] ? kept_values(dy, saved[1], "weight", N * ld[1], type) : saved[1];
+      const Tensor save = act != HOTK_ACT_NONE ? kept_values(dy, saved[2], "slopes", M * N, type == at::kFloat ? at::kFloat : at::kShort) : Tensor();
       if (M == 0) {
         if (wants & 1) dx = at::zeros(shape, x.options());
         if (wants & 2) dw = at::zeros({N, K}, x.options());

@@ -190,3 +190,50 @@ def test_piecewise_linear_slopes_are_exact():
             leaf = x.clone().requires_grad_(True)
             dx, = torch.autograd.grad(ops.linear_act(leaf, w, act=act), leaf, torch.ones(5, 1, dtype=dt, device=DEV))
             assert torch.equal(dx[:, 0], torch.tensor([low, low, low, 1., 1.]).to(dt).to(DEV))
+
+
+# ------------------------------------------------------------------------------------------------
+# what saved-tensor hooks give back
+# ------------------------------------------------------------------------------------------------
+def kept_leaves(M, K, N, dt, clone=False):
+    """operands that the forward pass copies (K no whole pieces, transposed), or takes in place"""
+    return [rnd(530, M, K + 9, dt=dt)[:, 3:K + 3], rnd(531, K, N, dt=dt).t(), rnd(532, N, dt=dt), rnd(533, M, N, dt=dt)]
+
+
+def kept_gradients(M, K, N, dt, mask):
+    from hot_amd import ops
+    x, w, b, r = [t.detach().requires_grad_(True) for t in kept_leaves(M, K, N, dt)]
+    kind = (torch.arange(M, device=DEV) % 3).to(torch.uint8) if mask else None
+    y = ops.linear_act(x, w, b, act='silu', residual=r)
+    z, h = ops.rms_norm(x, w[0], x, kind=kind)
+    return lambda: torch.autograd.grad((y, z, h), (x, w, b, r), (rnd(534, M, N, dt=dt), rnd(535, M, K, dt=dt), rnd(536, M, K, dt=dt)))
+
+
+@pytest.mark.parametrize('dt', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('mask', [False, True])
+@pytest.mark.parametrize('M,K,N', [(3, 742, 36), (70, 37, 24), (65, 64, 40), (1100, 40, 24)])
+def test_kept_tensors_in_another_layout(M, K, N, mask, dt):
+    """the same values at other strides: transposed storage, every second element of a row"""
+    def unpack(t):
+        if t.dim() == 2 and t.size(0) > 1:
+            return t.t().contiguous().t()
+        return torch.stack((t, torch.zeros_like(t)), -1)[..., 0]
+    want = kept_gradients(M, K, N, dt, mask)()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        got = kept_gradients(M, K, N, dt, mask)()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('change', [lambda t: t.to(torch.float64), lambda t: t[:-1], lambda t: t.cpu(), lambda t: torch.cat((t, t))])
+def test_kept_tensors_that_are_others_are_refused(change):
+    for which in range(7):                       # x, w, slopes of the product; stream, statistics, weight, kind of the norm
+        count = [0]
+
+        def unpack(t):
+            count[0] += 1
+            return change(t) if count[0] == which + 1 else t
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            gradients = kept_gradients(70, 37, 24, torch.float32, True)
+            with pytest.raises(RuntimeError, match='expected|kept for the backward pass|is on'):
+                gradients()
+                raise AssertionError(f'tensor {which} was taken')
