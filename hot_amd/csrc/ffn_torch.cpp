@@ -456,7 +456,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& weight, const optional<Tens
 
 struct LinearAct : torch::autograd::Function<LinearAct> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const optional<Tensor>& b, const optional<Tensor>& r,
-                        int64_t act) {
+                        int64_t act, int64_t dz_parts) {
     ctx->set_materialize_grads(false);
     Kept kept;
     const bool inner = wants_grad(x) || wants_grad(weight) || wants_grad(b);
@@ -465,6 +465,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     const bool own_x = !kept.x.t.is_same(x) && kept.x.n, own_w = !kept.w.t.is_same(weight);
     ctx->save_for_backward({own_x ? kept.x.t : x, own_w ? kept.w.t : weight, kept.save});
     ctx->saved_data["act"] = act;
+    ctx->saved_data["dz_parts"] = dz_parts;
     ctx->saved_data["shape"] = std::vector<int64_t>(x.sizes().begin(), x.sizes().end());
     ctx->saved_data["ld"] = std::vector<int64_t>{own_x ? kept.x.ld : 0, own_w ? kept.w.ld : 0};
     ctx->saved_data["wants"] = (int64_t)(wants_grad(x) | wants_grad(weight) << 1 | wants_grad(b) << 2 | wants_grad(r) << 3);
@@ -498,10 +499,12 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         // one pass over dy: dz where it is not dy itself, and its column sums
         Rows dz = gs;
         const bool itself = act == HOTK_ACT_NONE && whole(gs, N);
-        // dz is rounded to the type for the products, which adds as much error as the result's own rounding.  Where the products
-        // hide behind the launches around them the rest goes in too: up to 2^25 multiplications (1 to 5 us of the two products'
-        // 10 to 20, beside 50 that the host takes; at 2^28 it would be 7 of 14)
-        const bool two_parts = act != HOTK_ACT_NONE && type != at::kFloat && (double)M * N * K <= 33554432.;
+        // dz is rounded to the type for the products, which adds as much error as the result's own rounding; as two numbers of the
+        // type it leaves the result's alone, for twice the matrix work.  The caller says which, or (0) its size: two up to 2^25
+        // multiplications, where an eager call hides the second part behind its launches (1 to 5 us of the two products' 10 to 20,
+        // beside 50 that the host takes; a replayed graph pays them in full), and at 2^28 it would be 7 of 14
+        const int64_t parts = ctx->saved_data["dz_parts"].toInt();
+        const bool two_parts = act != HOTK_ACT_NONE && type != at::kFloat && (parts ? parts == 2 : (double)M * N * K <= 33554432.);
         if ((wants & 3) && !itself) {
           const int64_t ld = up(N, x.element_size());
           dz = {like(x, {two_parts ? 2 * M : M, ld}, type), ld, M, true};
@@ -536,16 +539,18 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         }
       }
     }
-    return {dx, dw, db, wants & 8 ? dy : Tensor(), Tensor()};
+    return {dx, dw, db, wants & 8 ? dy : Tensor(), Tensor(), Tensor()};
   }
 };
 
-Tensor linear_act(const Tensor& x, const Tensor& weight, const optional<Tensor>& b, const std::string& act, const optional<Tensor>& r) {
+Tensor linear_act(const Tensor& x, const Tensor& weight, const optional<Tensor>& b, const std::string& act, const optional<Tensor>& r,
+                  const optional<int64_t>& dz_parts) {
   check_input(x, "x");
+  if (dz_parts && *dz_parts != 1 && *dz_parts != 2) refuse("dz_parts: 1, 2 or None expected, got ", *dz_parts);
   const int code = act_code(act);
   check_linear(x, weight, b, r, x.scalar_type());
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(b) || wants_grad(r)))
-    return LinearAct::apply(x, weight, b, r, (int64_t)code);
+    return LinearAct::apply(x, weight, b, r, (int64_t)code, dz_parts.value_or(0));
   return linear_forward(x, weight, b, r, code, false, nullptr);
 }
 

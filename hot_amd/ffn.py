@@ -61,16 +61,21 @@ def quantize_rows(x):
         raise _wrong('quantize_rows', e) from None
 
 
-def linear_act(x, weight, bias=None, act='none', residual=None):
+def linear_act(x, weight, bias=None, act='none', residual=None, dz_parts=None):
     """y = act(x @ weight.T + bias) + residual in one product: x [..., K], weight [N, K] (torch.nn.Linear's layout), bias [N],
     residual and y [..., N], one type (fp32, bf16, fp16).  act: 'none', 'relu', 'leakyrelu' (slope 0.01), 'gelu' (by erf),
     'tanh', 'silu'.  Differentiable in x, weight, bias and residual.
+
+    dz_parts, for the gradients of bf16 and fp16 behind an activation: the two products take dz = dy act'(z) rounded to the type
+    (1: dx and dw are off by 1.4 times their own rounding) or as two numbers of the type (2: by their rounding alone, for twice the
+    matrix work).  None: two parts up to M N K = 2^25, one above, so a gradient's precision goes by the batch's size; name one
+    where it should not.
 
     Rows that start at 16-byte boundaries and hold whole 16-byte pieces (K a multiple of 8, of 4 in fp32) are read in place;
     others are copied once with zeros behind them; up to 64 rows of x, where the kernel for few rows is the faster one, are
     read at any alignment, and the weight with them.  Rows of up to 8 MiB, else HotkError."""
     try:
-        return (_binding or _ext()).linear_act(x, weight, bias, act, residual)
+        return (_binding or _ext()).linear_act(x, weight, bias, act, residual, dz_parts)
     except TypeError as e:
         raise _wrong('linear_act', e) from None
 

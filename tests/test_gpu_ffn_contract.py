@@ -237,3 +237,36 @@ def test_kept_tensors_that_are_others_are_refused(change):
             with pytest.raises(RuntimeError, match='expected|kept for the backward pass|is on'):
                 gradients()
                 raise AssertionError(f'tensor {which} was taken')
+
+
+# ------------------------------------------------------------------------------------------------
+# the precision of dz
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dt', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('M,N,K', [(50, 200, 130), (2000, 130, 72), (4096, 264, 136), (300, 1040, 1000)])
+def test_parts_of_dz(M, N, K, dt):
+    """whatever the size: in two parts the result's rounding is left (uniform in half a step, 0.58 u as a whole at most), in one
+    dz's beside it (0.82 u); None is one of the two, by the size"""
+    from hot_amd import ops
+    x, w, b, dy = rnd(540, M, K, dt=dt), rnd(541, N, K, dt=dt, scale=K ** -0.5), rnd(542, N, dt=dt), rnd(543, M, N, dt=dt)
+    dz = dy.double() * slope64(x.double() @ w.double().t() + b.double(), 'gelu')
+    want = (dz @ w.double(), dz.t() @ x.double())
+    x.requires_grad_(True), w.requires_grad_(True)
+    got = {parts: torch.autograd.grad(ops.linear_act(x, w, b, act='gelu', dz_parts=parts), (x, w), dy) for parts in (1, 2, None)}
+    for parts, most in ((1, 0.85), (2, 0.62)):
+        for what, g, v in zip(('dx', 'dw'), got[parts], want):
+            assert float((g.double() - v).norm() / v.norm()) <= most * half_step(dt), (what, parts)
+    assert all(torch.equal(a, c) for a, c in zip(got[None], got[2 if M * N * K <= 2 ** 25 else 1]))
+
+
+def test_parts_of_dz_that_do_not_matter():
+    """fp32, and no activation: dz is dy itself or held in fp32"""
+    from hot_amd import ops
+    from hot_amd._lib import HotkError
+    for dt, act in ((torch.float32, 'gelu'), (torch.bfloat16, 'none')):
+        x, w, dy = rnd(544, 30, 24, dt=dt).requires_grad_(True), rnd(545, 40, 24, dt=dt).requires_grad_(True), rnd(546, 30, 40, dt=dt)
+        one, two = (torch.autograd.grad(ops.linear_act(x, w, act=act, dz_parts=parts), (x, w), dy) for parts in (1, 2))
+        assert all(torch.equal(a, c) for a, c in zip(one, two))
+    for bad in (0, 3, -1, 1.5, 'one'):
+        with pytest.raises(HotkError):
+            ops.linear_act(x, w, dz_parts=bad)
