@@ -9,7 +9,8 @@ nothing else.  This module holds the pieces the three stacks share, written once
   * `pre_norm_block`, the LayerNorm -> Linear -> GELU -> Linear -> Dropout feed-forward block whose parameterised members
     sit at Sequential positions 0, 1 and 3 (keys `ffn.0.*`, `ffn.1.*`, `ffn.3.*`);
   * `norm_of`, the norm that a stack's norm='layernorm' | 'rmsnorm' names, and `feed_forward`, the block over plain rows with
-    RMSNorm: norm, product with GELU, product with the residual, each one kernel;
+    RMSNorm: norm, product with GELU, product with the residual, each one kernel (a block whose members have been replaced or
+    have hooks runs member by member);
   * `shared_feature_map`, the one FAVOR+ map an encoder hands to all its kernel-attention layers, and `maybe_redraw`.
 """
 from collections import namedtuple
@@ -18,6 +19,7 @@ import torch
 import torch.nn as nn
 
 from .. import ops
+from .._lib import HotkError
 from .common.kernel import KernelFeatureMap
 from .common.rmsnorm import RMSNorm
 
@@ -67,9 +69,31 @@ def norm_of(name, dim):
     return nn.LayerNorm(dim) if name == 'layernorm' else RMSNorm(dim)
 
 
+_MODULE_HOOKS = ('_forward_pre_hooks', '_forward_hooks', '_backward_pre_hooks', '_backward_hooks')
+
+
+def _plain_call(m, cls):
+    """calling m runs cls.forward and nothing else"""
+    return type(m) is cls and 'forward' not in m.__dict__ and not any(getattr(m, name) for name in _MODULE_HOOKS)
+
+
+def _as_assembled(ffn):
+    """the block is what pre_norm_block made of RMSNorm, nn.Linear, GELU by erf, nn.Linear and nn.Dropout, without hooks"""
+    everywhere = torch.nn.modules.module
+    return (_plain_call(ffn, nn.Sequential) and len(ffn) == 5
+            and all(_plain_call(m, cls) for m, cls in zip(ffn, (RMSNorm, nn.Linear, nn.GELU, nn.Linear, nn.Dropout))) and ffn[2].approximate == 'none'
+            and not any(getattr(everywhere, '_global' + name, None) for name in _MODULE_HOOKS))
+
+
 def feed_forward(ffn, x, residual=None, eight=None):
-    """h + ffn(h) for a pre_norm_block over rows with RMSNorm, nn.Linear and GELU, h = x (+ residual).  eight: the block's two
-    weights and their scales in 8 bits (quantize_block): the products then take 8-bit rows (no gradient)"""
+    """h + ffn(h) for a pre_norm_block over rows, h = x (+ residual); with the members that an encoder of norm='rmsnorm' gives it
+    three kernels, otherwise (a member replaced, or hooks on the block or a member) the block as it is called.  eight: the
+    block's two weights and their scales in 8 bits (quantize_block): the products then take 8-bit rows (no gradient)"""
+    if not _as_assembled(ffn):
+        if eight is not None:
+            raise HotkError('8-bit feed-forward products take the block as it was assembled: its members have been replaced, or hooks set')
+        h = x if residual is None else x + residual
+        return h + ffn(h)
     norm, first, _, second, drop = ffn
     if eight is not None:
         w1, s1, w2, s2 = eight
@@ -85,6 +109,8 @@ def feed_forward(ffn, x, residual=None, eight=None):
 
 def quantize_block(ffn):
     """a block's weights for feed_forward(eight=...): 8 bits with one scale per output column"""
+    if not _as_assembled(ffn):
+        raise HotkError('8-bit feed-forward products take the block as it was assembled: its members have been replaced, or hooks set')
     with torch.no_grad():
         return (*ops.quantize_rows(ffn[1].weight), *ops.quantize_rows(ffn[3].weight))
 

@@ -53,7 +53,8 @@ class EncLayer(nn.Module):
     def quantize_feed_forward(self):
         """keep the feed-forward weights in 8 bits too, for calls in eval mode without gradients; taken from the weights as they
         are now: a forward call that finds them changed, moved or replaced since raises (values written through .data are not
-        seen).  They are part of neither the state_dict nor a copy or pickle of the module, which serve the full weights"""
+        seen).  They are part of neither the state_dict nor a copy or pickle of the module, which serve the full weights.  A block whose members
+        have been replaced or have hooks raises, here and in such a forward call"""
         if self.norm != 'rmsnorm':
             raise HotkError("8-bit feed-forward products need norm='rmsnorm'")
         for name, t in zip(_EIGHT, _stack.quantize_block(self.ffn)):
@@ -61,7 +62,7 @@ class EncLayer(nn.Module):
         self._eight_of = [(w, w.data_ptr(), w._version) for w in self._ffn_weights()]
 
     def _ffn_weights(self):
-        return self.ffn[1].weight, self.ffn[3].weight
+        return [getattr(m, 'weight', None) for m in list(self.ffn.children())[1:4:2]]
 
     def __getstate__(self):
         state = self.__dict__.copy()
