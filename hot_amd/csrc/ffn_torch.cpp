@@ -286,17 +286,17 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
       const Rows hs = rows(h), gs = rows(dy), ss = dh.defined() ? rows(dh) : Rows{};
       void* st = stream_of(h);
       int64_t parts = 0;
-      check(L.rmsnorm_partials(hs.n, D, ty, &parts), "hotk_rmsnorm_partials");
+      if (wants & 2) {
+        check(L.rmsnorm_partials(hs.n, D, ty, &parts), "hotk_rmsnorm_partials");
+        dw = like(h, {D}, type);
+      }
       dx = like(h);
       const Tensor part = parts ? like(h, {parts, D}, at::kFloat) : Tensor();
-      if (wants & 2) dw = like(h, {D}, h.scalar_type());
       launch("hotk_rmsnorm_bwd", (dh.defined() ? 4 : 3) * h.numel() * h.element_size(), [&] {
         return L.rmsnorm_bwd(gs.p(), gs.ld, ss.p(), ss.ld, hs.p(), hs.ld, rstd.const_data_ptr<float>(), w.const_data_ptr(), kind_ptr(kind),
                              (unsigned)keep, dx.data_ptr(), (float*)out(part), parts ? nullptr : out(dw), hs.n, D, ty, st);
       });
-      if ((wants & 2) && parts) {
-        launch("hotk_sum_partials", 4 * parts * D, [&] { return L.sum_partials(part.const_data_ptr<float>(), parts, D, dw.data_ptr(), ty, st); });
-      }
+      if (parts) launch("hotk_sum_partials", 4 * parts * D, [&] { return L.sum_partials(part.const_data_ptr<float>(), parts, D, dw.data_ptr(), ty, st); });
     }
     return {wants & 1 ? dx : Tensor(), dw, wants & 4 ? dx : Tensor(), Tensor(), Tensor(), Tensor()};
   }

@@ -485,7 +485,7 @@ extern "C" int hotk_rmsnorm_bwd(const void* dy, int64_t ld_dy, const void* dh, i
                                 void* dw, int64_t R, int64_t D, int type, void* stream) {
   HOTK_CHECK_ARG(R >= 0);
   if (!hotk_rmsnorm_supported(D, type)) return HOTK_EUNSUPPORTED;
-  HOTK_CHECK_ARG(rn_few(R, D, ffn_bytes(type)) ? !partial : partial && !dw);
+  HOTK_CHECK_ARG(rn_few(R, D, ffn_bytes(type)) ? !partial : !dw);
   HOTK_CHECK_ARG(!dw || ffn_elem_aligned(dw, type));
   HOTK_CHECK_ARG(R == 0 || (rn_rows_ok(dy, ld_dy, D, type) && rn_rows_ok(h, ld_h, D, type) && rstd && rn_rows_ok(dx, D, D, type)));
   HOTK_CHECK_ARG(rn_rows_ok(w, D, D, type) && (!dh || rn_rows_ok(dh, ld_dh, D, type)));

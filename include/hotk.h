@@ -527,7 +527,7 @@ int hotk_rmsnorm_quant(const void* x, int64_t ld_x, const void* res, int64_t ld_
 int hotk_quantize_rows(const void* x, int64_t ld_x, uint8_t* q, float* scale, int64_t R, int64_t D, int type, void* stream);
 /* dx[r] (the gradient of x and of res) from dy, the gradient dh of h (NULL: none), h and rstd; n = hotk_rmsnorm_partials(R, D,
  * type): partial[n][D], dw's partial sums, added up in order by hotk_sum_partials; where n is 0 (few rows) partial is NULL and
- * dw (NULL: not wanted) is written itself */
+ * dw is written itself.  Both NULL: dw is not wanted */
 int hotk_rmsnorm_partials(int64_t R, int64_t D, int type, int64_t* n_partials);
 int hotk_rmsnorm_bwd(const void* dy, int64_t ld_dy, const void* dh, int64_t ld_dh, const void* h, int64_t ld_h,
                      const float* rstd, const void* w, const uint8_t* kind, unsigned keep, void* dx, float* partial, void* dw,

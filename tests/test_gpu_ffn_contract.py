@@ -270,3 +270,24 @@ def test_parts_of_dz_that_do_not_matter():
     for bad in (0, 3, -1, 1.5, 'one'):
         with pytest.raises(HotkError):
             ops.linear_act(x, w, dz_parts=bad)
+
+
+# ------------------------------------------------------------------------------------------------
+# gradients that nobody asked for
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dt', TYPES)
+@pytest.mark.parametrize('R,D', [(3, 40), (1024, 40), (1025, 40), (2100, 7), (1500, 520), (1030, 20000)])
+def test_norm_gradient_of_the_rows_alone(R, D, dt):
+    """a frozen weight: dx as with the weight's gradient, and no memory or launch for the latter"""
+    from hot_amd import _lib, ops
+    x, w, dy = rnd(550, R, D, dt=dt).requires_grad_(True), rnd(551, D, dt=dt), rnd(552, R, D, dt=dt)
+    want, _ = torch.autograd.grad(ops.rms_norm(x, v := w.clone().requires_grad_(True)), (x, v), dy)
+    y = ops.rms_norm(x, w)
+    requested = lambda: torch.cuda.memory_stats()['requested_bytes.all.allocated']      # (blocks may be larger than asked for)
+    before = requested()
+    _lib.timing_begin(None)
+    got, = torch.autograd.grad(y, x, dy)
+    seen = _lib.timing_end()
+    asked = requested() - before
+    assert asked == got.numel() * got.element_size()                                    # the result and nothing else
+    assert torch.equal(got, want) and set(seen) == {'hotk_rmsnorm_bwd'}
