@@ -291,3 +291,42 @@ def test_norm_gradient_of_the_rows_alone(R, D, dt):
     asked = requested() - before
     assert asked == got.numel() * got.element_size()                                    # the result and nothing else
     assert torch.equal(got, want) and set(seen) == {'hotk_rmsnorm_bwd'}
+
+
+# ------------------------------------------------------------------------------------------------
+# gradients past 2^31 elements: operands of -1, 0 and 1, so that every sum is a whole number below 2^24 and exact in any order
+# ------------------------------------------------------------------------------------------------
+def whole(seed, *size):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.randint(-1, 2, size, generator=g, device=DEV, dtype=torch.int8).to(torch.bfloat16)
+
+
+ROWS, CHUNK = 1100000, 55000
+
+
+def test_weight_gradient_past_32_bits():
+    """dw = dy^T x with x of 2^31 elements, contracted down its columns in splits: bit for bit"""
+    from hot_amd import ops
+    x, V, dy = whole(560, ROWS, 2048), whole(561, 16, 2048).requires_grad_(True), whole(562, ROWS, 16)
+    dV, = torch.autograd.grad(ops.linear_act(x, V), V, dy)
+    want = torch.zeros(16, 2048, device=DEV, dtype=torch.float64)
+    for i in range(0, ROWS, CHUNK):
+        want += dy[i:i + CHUNK].double().t().contiguous() @ x[i:i + CHUNK].double()
+    assert torch.equal(dV, want.to(torch.bfloat16))
+
+
+def test_all_gradients_past_32_bits():
+    """dy, slopes and dz of 2^31 elements each"""
+    from hot_amd import ops
+    x, W, b, dy = whole(563, ROWS, 24), whole(564, 2048, 24), whole(565, 2048), whole(566, ROWS, 2048)
+    leaves = [t.requires_grad_(True) for t in (x, W, b)]
+    dx, dW, db = torch.autograd.grad(ops.linear_act(*leaves, act='relu'), leaves, dy)
+    want_w, want_b = torch.zeros(2048, 24, device=DEV, dtype=torch.float64), torch.zeros(2048, device=DEV, dtype=torch.float64)
+    Wd = W.detach().double()
+    for i in range(0, ROWS, CHUNK):
+        xd = x.detach()[i:i + CHUNK].double()
+        dz = dy[i:i + CHUNK].double() * (xd @ Wd.t().contiguous() + b.detach().double() > 0)
+        want_w += dz.t().contiguous() @ xd
+        want_b += dz.sum(0)
+        assert torch.equal(dx[i:i + CHUNK], (dz @ Wd).to(torch.bfloat16)), i
+    assert torch.equal(dW, want_w.to(torch.bfloat16)) and torch.equal(db, want_b.to(torch.bfloat16))
