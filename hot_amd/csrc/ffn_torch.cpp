@@ -362,6 +362,15 @@ Rows padded(const Rows& in, int64_t C) {   // itself where it is whole, else a c
   return {o, ld, in.n, true};
 }
 
+// operands of a product: its tiles reach rows by 32-bit offsets, at strides of up to 8 MiB; short rows further apart are copied
+constexpr int64_t MAX_ROW_BYTES = 1 << 23;
+Rows operand(const Tensor& t) {
+  const Rows r = rows(t);
+  const int64_t e = t.element_size(), C = t.size(-1);
+  if (r.ld * e <= MAX_ROW_BYTES || C * e > MAX_ROW_BYTES) return r;
+  return {r.t.clone(at::MemoryFormat::Contiguous), C, r.n};
+}
+
 struct Extras {
   Tensor bias, save, x_scale, w_scale;
   Rows res;
@@ -439,7 +448,7 @@ Tensor linear_forward(const Tensor& x, const Tensor& weight, const optional<Tens
                       Kept* kept) {
   const c10::DeviceGuard guard(x.device());
   const int64_t K = x.size(-1), N = weight.size(0);
-  const Rows xs = rows(x), ws = rows(weight);
+  const Rows xs = operand(x), ws = operand(weight);
   Extras e;
   e.act = act;
   if (b) e.bias = b->contiguous();
@@ -494,7 +503,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         if (wants & 2) dw = at::zeros({N, K}, x.options());
         if (wants & 4) db = at::zeros({N}, x.options());
       } else {
-        const Rows gs = rows(dy);
+        const Rows gs = operand(dy);
         const int ty = type_of(type);
         // one pass over dy: dz where it is not dy itself, and its column sums
         Rows dz = gs;
@@ -531,11 +540,11 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         e.x_lo = lo;
         if (wants & 1) {
           e.flags = HOTK_LINEAR_W_DOWN;
-          dx = product(dz, padded(ld[1] ? Rows{weight, ld[1], N, true} : rows(weight), K), M, K, N, shape, type, e);
+          dx = product(dz, padded(ld[1] ? Rows{weight, ld[1], N, true} : operand(weight), K), M, K, N, shape, type, e);
         }
         if (wants & 2) {
           e.flags = HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN;
-          dw = product(dz, padded(ld[0] ? Rows{x, ld[0], M, true} : rows(x), K), N, K, M, {N, K}, type, e);
+          dw = product(dz, padded(ld[0] ? Rows{x, ld[0], M, true} : operand(x), K), N, K, M, {N, K}, type, e);
         }
       }
     }
@@ -573,7 +582,7 @@ Tensor linear_act_quantized(const Tensor& xq, const Tensor& x_scale, const Tenso
   e.res = rows(r);
   e.x_scale = x_scale.contiguous();
   e.w_scale = w_scale.contiguous();
-  return product(rows(xq), rows(wq), xq.numel() / K, wq.size(0), K, result_shape(xq, wq.size(0)), type, e);
+  return product(operand(xq), operand(wq), xq.numel() / K, wq.size(0), K, result_shape(xq, wq.size(0)), type, e);
 }
 
 }  // namespace

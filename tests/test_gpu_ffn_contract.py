@@ -330,3 +330,29 @@ def test_all_gradients_past_32_bits():
         want_b += dz.sum(0)
         assert torch.equal(dx[i:i + CHUNK], (dz @ Wd).to(torch.bfloat16)), i
     assert torch.equal(dW, want_w.to(torch.bfloat16)) and torch.equal(db, want_b.to(torch.bfloat16))
+
+
+# ------------------------------------------------------------------------------------------------
+# rows that lie far apart, rows that are too long
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dt', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('M', [3, 70])
+def test_short_rows_far_apart(M, dt):
+    """a stride above 8 MiB is no reason to refuse rows of 40 elements"""
+    from hot_amd import ops
+    far = (1 << 23) // dt.itemsize + 64
+    x, w, dy = rnd(570, M, 40, dt=dt), rnd(571, 5, 40, dt=dt), rnd(572, M, 24, dt=dt)
+    W = rnd(573, 24, 40, dt=dt)
+
+    def apart(t):
+        big = torch.empty(t.size(0), far, dtype=dt, device=DEV)[:, 8:8 + t.size(1)]
+        return big.copy_(t)
+    def grads(x, W, dy):
+        x, W = x.detach().requires_grad_(True), W.detach().requires_grad_(True)
+        y = ops.linear_act(x, W, act='gelu')
+        return (y.detach(),) + torch.autograd.grad(y, (x, W), dy)
+    want = grads(x, W, dy)
+    assert all(torch.equal(a, b) for a, b in zip(grads(apart(x), W, apart(dy)), want))
+    assert all(torch.equal(a, b) for a, b in zip(grads(x, apart(W), dy), want))
+    dx, = torch.autograd.grad(ops.linear_act(v := x.clone().requires_grad_(True), W), v, apart(dy))      # dz is dy, in place or copied
+    assert torch.equal(dx, torch.autograd.grad(ops.linear_act(v := x.clone().requires_grad_(True), W), v, dy)[0])
