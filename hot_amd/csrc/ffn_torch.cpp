@@ -469,6 +469,8 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     ctx->set_materialize_grads(false);
     Kept kept;
     const bool inner = wants_grad(x) || wants_grad(weight) || wants_grad(b);
+    if ((wants_grad(x) || wants_grad(weight)) && up(weight.size(0), x.element_size()) * x.element_size() > MAX_ROW_BYTES)
+      refuse("gradients of rows of up to 8 MiB: the result's rows have ", weight.size(0), " elements");      // (now, not in the backward pass)
     const Tensor y = linear_forward(x, weight, b, r, (int)act, inner, &kept);
     // the input itself where it was read in place (so that a later change of it is noticed), else the copy
     const bool own_x = !kept.x.t.is_same(x) && kept.x.n, own_w = !kept.w.t.is_same(weight);

@@ -73,8 +73,8 @@ def linear_act(x, weight, bias=None, act='none', residual=None, dz_parts=None):
 
     Rows that start at 16-byte boundaries and hold whole 16-byte pieces (K a multiple of 8, of 4 in fp32) are read in place;
     others are copied once with zeros behind them; up to 64 rows of x, where the kernel for few rows is the faster one, are
-    read at any alignment, and the weight with them.  Rows of x and weight hold up to 8 MiB, else HotkError;
-    shorter rows that lie further apart are copied."""
+    read at any alignment, and the weight with them.  Rows of x and weight hold up to 8 MiB, those of y too where x or weight has a
+    gradient, else HotkError; shorter rows that lie further apart are copied."""
     try:
         return (_binding or _ext()).linear_act(x, weight, bias, act, residual, dz_parts)
     except TypeError as e:

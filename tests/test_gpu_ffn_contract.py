@@ -356,3 +356,19 @@ def test_short_rows_far_apart(M, dt):
     assert all(torch.equal(a, b) for a, b in zip(grads(x, apart(W), dy), want))
     dx, = torch.autograd.grad(ops.linear_act(v := x.clone().requires_grad_(True), W), v, apart(dy))      # dz is dy, in place or copied
     assert torch.equal(dx, torch.autograd.grad(ops.linear_act(v := x.clone().requires_grad_(True), W), v, dy)[0])
+
+
+def test_gradients_of_too_long_results_are_refused_at_once():
+    from hot_amd import ops
+    from hot_amd._lib import HotkError
+    N = (1 << 22) + 8
+    x, w = rnd(574, 2, 1, dt=torch.bfloat16), torch.ones(N, 1, dtype=torch.bfloat16, device=DEV)
+    assert torch.equal(ops.linear_act(x, w), x.expand(2, N))
+    for which in (x, w):
+        which.requires_grad_(True)
+        with pytest.raises(HotkError, match='8 MiB'):
+            ops.linear_act(x, w)
+        which.requires_grad_(False)
+    b = torch.zeros(N, dtype=torch.bfloat16, device=DEV, requires_grad=True)       # the bias's alone needs no product
+    db, = torch.autograd.grad(ops.linear_act(x, w, b), b, torch.ones(2, N, dtype=torch.bfloat16, device=DEV))
+    assert (db == 2).all()
