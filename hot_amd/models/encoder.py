@@ -6,7 +6,7 @@ hot_pytorch/models/encoder.py:20-96; the assembly is table-driven (models/_stack
 readout SelfAttn(., 0) for an order-0 output, which is linear in |E|.  Quadratic softmax attention for output orders >= 1
 (att_cfg='default') is outside the linear-cost path: NotImplementedError.  The dense layout has the same readout
 (models/dense/attn.py).  norm='rmsnorm' (not in the reference; the default is its LayerNorm) takes root-mean-square norms
-instead, with the padding mask in the same kernel."""
+instead; in the sparse layout a norm that stands alone in its Apply has the padding mask in the same kernel."""
 import torch.nn as nn
 
 from . import _stack
