@@ -979,7 +979,6 @@ extern "C" int hotk_linear_act(const hotk_linear_args* args, void* workspace, si
   ffn_dispatch(args->out_type, [&](auto* tag) {
     using OT = std::remove_pointer_t<decltype(tag)>;
     using T8 = std::conditional_t<std::is_same<OT, float>::value, e4m3_wide, e4m3>;
-      using T8 = std::conditional_t<std::is_same<OT, float>::value, e4m3_wide, e4m3>;
     rc = args->type == HOTK_E4M3 ? la_product<T8, OT, false, false>(*args, workspace, ws_bytes, st)
        : !(args->flags & HOTK_LINEAR_W_DOWN) ? la_product<OT, OT, false, false>(*args, workspace, ws_bytes, st)
        : !(args->flags & HOTK_LINEAR_X_DOWN) ? la_product<OT, OT, false, true>(*args, workspace, ws_bytes, st)
