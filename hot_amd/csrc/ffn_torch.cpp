@@ -472,9 +472,10 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     if ((wants_grad(x) || wants_grad(weight)) && up(weight.size(0), x.element_size()) * x.element_size() > MAX_ROW_BYTES)
       refuse("gradients of rows of up to 8 MiB: the result's rows have ", weight.size(0), " elements");      // (now, not in the backward pass)
     const Tensor y = linear_forward(x, weight, b, r, (int)act, inner, &kept);
-    // the input itself where it was read in place (so that a later change of it is noticed), else the copy
+    // what a gradient needs: x for the weight's, the weight for x's; the input itself where it was read in place (so that a later
+    // change of it is noticed), else the copy
     const bool own_x = !kept.x.t.is_same(x) && kept.x.n, own_w = !kept.w.t.is_same(weight);
-    ctx->save_for_backward({own_x ? kept.x.t : x, own_w ? kept.w.t : weight, kept.save});
+    ctx->save_for_backward({!wants_grad(weight) ? Tensor() : own_x ? kept.x.t : x, !wants_grad(x) ? Tensor() : own_w ? kept.w.t : weight, kept.save});
     ctx->saved_data["act"] = act;
     ctx->saved_data["dz_parts"] = dz_parts;
     ctx->saved_data["shape"] = std::vector<int64_t>(x.sizes().begin(), x.sizes().end());
@@ -494,16 +495,17 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
       const c10::DeviceGuard guard(dy.device());
       const auto type = dy.scalar_type();
       const int64_t K = shape.back(), N = dy.size(-1), M = dy.numel() / N;
-      // the operands: themselves in any layout, or copies of rows `ld` apart
-      if (!ld[0]) check_with(dy, saved[0], "x", shape, type);
-      if (!ld[1]) check_with(dy, saved[1], "weight", {N, K}, type);
-      const Tensor x = ld[0] ? kept_values(dy, saved[0], "x", M * ld[0], type) : saved[0];
-      const Tensor weight = ld[1] ? kept_values(dy, saved[1], "weight", N * ld[1], type) : saved[1];
+      // an operand: itself in any layout, or a copy of rows `ld` apart
+      const auto kept = [&](int i, const char* what, at::IntArrayRef own, int64_t n) {
+        if (ld[i]) return Rows{kept_values(dy, saved[i], what, n * ld[i], type), ld[i], n, true};
+        check_with(dy, saved[i], what, own, type);
+        return operand(saved[i]);
+      };
       const Tensor save = act != HOTK_ACT_NONE ? kept_values(dy, saved[2], "slopes", M * N, type == at::kFloat ? at::kFloat : at::kShort) : Tensor();
       if (M == 0) {
-        if (wants & 1) dx = at::zeros(shape, x.options());
-        if (wants & 2) dw = at::zeros({N, K}, x.options());
-        if (wants & 4) db = at::zeros({N}, x.options());
+        if (wants & 1) dx = at::zeros(shape, dy.options());
+        if (wants & 2) dw = at::zeros({N, K}, dy.options());
+        if (wants & 4) db = at::zeros({N}, dy.options());
       } else {
         const Rows gs = operand(dy);
         const int ty = type_of(type);
@@ -517,36 +519,36 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         const int64_t parts = ctx->saved_data["dz_parts"].toInt();
         const bool two_parts = act != HOTK_ACT_NONE && type != at::kFloat && (parts ? parts == 2 : (double)M * N * K <= 33554432.);
         if ((wants & 3) && !itself) {
-          const int64_t ld = up(N, x.element_size());
-          dz = {like(x, {two_parts ? 2 * M : M, ld}, type), ld, M, true};
+          const int64_t ld = up(N, dy.element_size());
+          dz = {like(dy, {two_parts ? 2 * M : M, ld}, type), ld, M, true};
         }
         Tensor part;
         if (wants & 4) {
           int64_t n = 0;
           check(L.linear_dz_partials(M, &n), "hotk_linear_dz_partials");
-          db = like(x, {N}, type);
-          if (n > 1) part = like(x, {n, N}, at::kFloat);
+          db = like(dy, {N}, type);
+          if (n > 1) part = like(dy, {n, N}, at::kFloat);
         }
         const bool write = (wants & 3) && !itself;
-        void* lo = write && two_parts ? (char*)dz.t.data_ptr() + M * dz.ld * x.element_size() : nullptr;
+        void* lo = write && two_parts ? (char*)dz.t.data_ptr() + M * dz.ld * dy.element_size() : nullptr;
         if (write || db.defined())
-          launch("hotk_linear_dz", M * N * x.element_size() * (1 + write + (act != HOTK_ACT_NONE)), [&] {
+          launch("hotk_linear_dz", M * N * dy.element_size() * (1 + write + (act != HOTK_ACT_NONE)), [&] {
             return L.linear_dz(gs.p(), gs.ld, out(save), act, write ? dz.t.data_ptr() : nullptr, lo, dz.ld, (float*)out(part), part.defined() ? nullptr : out(db),
-                               M, N, ty, stream_of(x));
+                               M, N, ty, stream_of(dy));
           });
         if (part.defined())
           launch("hotk_sum_partials", 4 * part.numel(), [&] {
-            return L.sum_partials(part.const_data_ptr<float>(), part.size(0), N, db.data_ptr(), ty, stream_of(x));
+            return L.sum_partials(part.const_data_ptr<float>(), part.size(0), N, db.data_ptr(), ty, stream_of(dy));
           });
         Extras e;
         e.x_lo = lo;
         if (wants & 1) {
           e.flags = HOTK_LINEAR_W_DOWN;
-          dx = product(dz, padded(ld[1] ? Rows{weight, ld[1], N, true} : operand(weight), K), M, K, N, shape, type, e);
+          dx = product(dz, padded(kept(1, "weight", {N, K}, N), K), M, K, N, shape, type, e);
         }
         if (wants & 2) {
           e.flags = HOTK_LINEAR_X_DOWN | HOTK_LINEAR_W_DOWN;
-          dw = product(dz, padded(ld[0] ? Rows{x, ld[0], M, true} : operand(x), K), N, K, M, {N, K}, type, e);
+          dw = product(dz, padded(kept(0, "x", shape, M), K), N, K, M, {N, K}, type, e);
         }
       }
     }

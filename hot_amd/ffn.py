@@ -33,7 +33,8 @@ def rms_norm(x, weight, residual=None, eps=1e-6, kind=None, keep=KEEP_VALID):
     type as the stream is stored, and the result is (y, h).
 
     x, residual [..., D], weight [D], one type (fp32, bf16, fp16), D <= 32768.  kind (uint8, one per row: a plan's `kind` or
-    `nkind`) and keep: rows that keep leaves out are not read, and are zero in y, h and the gradients.  Differentiable in x,
+    `nkind`) and keep: rows that keep leaves out are not read, and are zero in y, h and the gradients.  The squares are added up in
+    fp32: a row whose sum of squares passes its range (3e38, elements of some 1e18) comes out as zeros.  Differentiable in x,
     weight and residual."""
     try:
         return (_binding or _ext()).rms_norm(x, weight, residual, eps, kind, keep)

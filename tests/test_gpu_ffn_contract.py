@@ -372,3 +372,47 @@ def test_gradients_of_too_long_results_are_refused_at_once():
     b = torch.zeros(N, dtype=torch.bfloat16, device=DEV, requires_grad=True)       # the bias's alone needs no product
     db, = torch.autograd.grad(ops.linear_act(x, w, b), b, torch.ones(2, N, dtype=torch.bfloat16, device=DEV))
     assert (db == 2).all()
+
+
+# ------------------------------------------------------------------------------------------------
+# what is kept for the backward pass
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('K', [40, 37])
+@pytest.mark.parametrize('M', [6, 200])
+def test_only_what_a_gradient_needs_is_kept(M, K):
+    """x is kept for the weight's gradient and the weight for x's, so the other one may change or go in between; one that is needed and
+    read in place may not"""
+    from hot_amd import ops
+    dt = torch.bfloat16
+    x0, w0, b0, dy = rnd(580, M, K, dt=dt), rnd(581, 24, K, dt=dt), rnd(582, 24, dt=dt), rnd(583, M, 24, dt=dt)
+    full = [t.clone().requires_grad_(True) for t in (x0, w0, b0)]
+    want = torch.autograd.grad(ops.linear_act(*full, act='gelu'), full, dy)
+    for which in range(3):
+        leaves = [t.clone().requires_grad_(i == which) for i, t in enumerate((x0, w0, b0))]
+        y = ops.linear_act(*leaves, act='gelu')
+        needed = {0: 1, 1: 0}.get(which)
+        for i, t in enumerate(leaves):
+            if i not in (which, needed):
+                t.add_(1)
+        got, = torch.autograd.grad(y, leaves[which], dy)
+        assert torch.equal(got, want[which]), which
+    if K % 8 == 0:
+        for which, other in ((0, 1), (1, 0)):
+            leaves = [t.clone().requires_grad_(i == which) for i, t in enumerate((x0, w0, b0))]
+            y = ops.linear_act(*leaves, act='gelu')
+            leaves[other].add_(1)
+            with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+                torch.autograd.grad(y, leaves[which], dy)
+
+
+def test_rows_before_a_frozen_weight_are_not_held():
+    from hot_amd import ops
+    x, w = torch.zeros(1 << 20, 64, device=DEV, requires_grad=True), rnd(584, 8, 64)
+    x1 = x * 1
+    before = torch.cuda.memory_allocated()
+    y = ops.linear_act(x1, w)
+    del x1
+    assert before - torch.cuda.memory_allocated() >= (1 << 28) - y.numel() * 4 - (1 << 22)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    want = w.double().sum(0)
+    hold('dx', dx[:3], want.expand(3, 64), 10 * E * w.double().abs().sum(0).expand(3, 64))
