@@ -23,12 +23,12 @@
 // barrier the DMA of the step after next starts and the next step's first fragments are read while matrix instructions run.
 //
 // Measured (large library products reach 1 354 TFLOP/s in bf16, 2 748 in e4m3, 153 in fp32 here): 8 192^3 bf16 807 us =
-// 1 362 TFLOP/s, 8 192^3 e4m3 389 us = 2 823; 16 384 x 4 096 x 1 024 bf16 129 us = 1 066 (with bias, gelu and slopes 184), its
+// 1 362 TFLOP/s, 8 192^3 e4m3 389 us = 2 823; 16 384 x 4 096 x 1 024 bf16 129 us = 1 066 (with bias, gelu and slopes 190), its
 // dx 111 us = 1 238, its dw 135 us = 1 018; 8 192 x 2 048 x 4 096 e4m3 62 us = 2 200; 4 096 x 4 096 x 1 024 fp32 254 us = 135.
 //
-// For training, 16-bit types keep f'(z) in a 16-bit code (la_slope_codes) whose error stays below what dz's own rounding adds,
-// where z rounded to the type would add as much again and more as |z| grows, and the backward pass needs no transcendental.
-// fp32 keeps z.
+// For training, 16-bit types keep f'(z) in a 16-bit code (la_slope_codes) whose half step stays below the type's for slopes
+// down to 2^-15 (fp16) and 2^-58 (bf16), where z rounded to the type would add as much as dz's rounding and more as |z| grows,
+// and the backward pass needs no transcendental.  fp32 keeps z.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -123,7 +123,7 @@ __device__ __forceinline__ void la_times_slope(f32x4& v, const f32x4& z, int act
 // Codes of slopes, -0.13 < d < 1.13.  A code is sign(d) k - 8192: the codes below zero that negative slopes leave unused go to the
 // positive ones.  From |d| = 1/16 up k goes in steps of 2^-14 (2^-11 of |d| at most); below, where a saturated unit's gradient
 // lives, as a root of |d|, so that k's half step stays small against |d|:  k = 21504 (16 |d|)^(1/n).  fp16: n = 8, half a step is
-// 2^-12.4 of |d| at 1/16, 2^-11.2 at 2^-14 (fp16's smallest normal number), 2^-10 at 2^-23; bf16: n = 16, 2^-11.4 at 1/16, 2^-10 at
+// 2^-12.4 of |d| at 1/16, 2^-11.1 at 2^-14 (fp16's smallest normal number), 2^-10 at 2^-23; bf16: n = 16, 2^-11.4 at 1/16, 2^-10 at
 // 2^-26, 2^-8 at 2^-58.  The types' own half steps are 2^-11 and 2^-8.  (With one step of 2^-14 for all, at the cost of two
 // transcendentals less, gradients of tanh units were 9 % off at |z| = 5.5 and zero from 6 on.)  Piecewise linear activations
 // need one bit.

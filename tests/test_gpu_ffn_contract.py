@@ -416,3 +416,53 @@ def test_rows_before_a_frozen_weight_are_not_held():
     dx, = torch.autograd.grad(y, x, torch.ones_like(y))
     want = w.double().sum(0)
     hold('dx', dx[:3], want.expand(3, 64), 10 * E * w.double().abs().sum(0).expand(3, 64))
+
+
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_under_checkpointing(reentrant):
+    """the forward pass run again in the backward pass, with its own kept tensors: the same gradients"""
+    from torch.utils.checkpoint import checkpoint
+    from hot_amd import ops
+    M, K, N, dt = 70, 37, 24, torch.bfloat16
+
+    def step(x, w, b, r):
+        return ops.linear_act(ops.rms_norm(x, w[0]), w, b, act='gelu', residual=r)
+    def gradients(call):
+        leaves = [t.detach().clone().requires_grad_(True) for t in kept_leaves(M, K, N, dt)]
+        return torch.autograd.grad(call(*leaves), leaves, rnd(590, M, N, dt=dt)) if not reentrant else backward(call, leaves)
+    def backward(call, leaves):
+        call(*leaves).backward(rnd(590, M, N, dt=dt))
+        return [t.grad for t in leaves]
+    got, want = gradients(lambda *t: checkpoint(step, *t, use_reentrant=reentrant)), gradients(step)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('parts', [1, 2])
+def test_parts_of_dz_in_a_graph(parts):
+    """captured forward and backward, replayed with other eager work between: each replay equals the eager result"""
+    from hot_amd import ops
+    dt = torch.float16
+    x, w, b, dy = rnd(591, 300, 136, dt=dt), rnd(592, 264, 136, dt=dt, scale=0.1), rnd(593, 264, dt=dt), rnd(594, 300, 264, dt=dt)
+
+    def step():
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        y = ops.linear_act(*leaves, act='silu', dz_parts=parts)
+        return [y.detach()] + list(torch.autograd.grad(y, leaves, dy))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for turn in range(3):
+        x.copy_(rnd(595 + turn, 300, 136, dt=dt))
+        want = [t.clone() for t in step()]
+        for t in out:
+            t.zero_()
+        g.replay()
+        step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(out, want)), turn
