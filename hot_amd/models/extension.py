@@ -53,8 +53,8 @@ class EncLayer(nn.Module):
     def quantize_feed_forward(self):
         """keep the feed-forward weights in 8 bits too, for calls in eval mode without gradients; taken from the weights as they
         are now: a forward call that finds them changed, moved or replaced since raises (values written through .data are not
-        seen).  They are part of neither the state_dict nor a copy or pickle of the module, which serve the full weights.  A block whose members
-        have been replaced or have hooks raises, here and in such a forward call"""
+        seen).  A block whose members have been replaced or have hooks raises, here and in such a call.  The 8-bit weights are
+        part of neither the state_dict nor a copy or pickle of the module, which serve the full weights"""
         if self.norm != 'rmsnorm':
             raise HotkError("8-bit feed-forward products need norm='rmsnorm'")
         for name, t in zip(_EIGHT, _stack.quantize_block(self.ffn)):
